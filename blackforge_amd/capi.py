@@ -138,6 +138,14 @@ SIGNATURES = {
     "bf_hip_rmsnorm_feedforward_bf16": [P, P, P, P, P, ctypes.c_int, P, c_size, c_size, c_size, ctypes.c_int, S],
     "bf_hip_attention_backward_img": [P, P, P, P, P, P, P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, c_float,
                                       c_size, S],
+    "bf_hip_attention_tree": [P, P, P, P, P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, c_float, S],
+    "bf_hip_attention_tree_weights": [P, P, P, P, P, P, P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, c_size, c_float, S],
+    "bf_hip_attention_key_weights": [P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, c_size, c_size, c_float, c_size, c_size,
+                                     S],
+    "bf_hip_kv_evict": [P, P, P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, c_size, c_size, S],
+    "bf_hip_tree_accept": [P, P, P, P, P, P, P, c_size, c_size, c_size, S],
+    "bf_hip_kv_commit": [ctypes.POINTER(c_ptr), ctypes.POINTER(c_ptr), ctypes.POINTER(c_ptr), ctypes.POINTER(c_ptr), ctypes.POINTER(c_ptr), c_size,
+                         P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_size, S],
     "bf_hip_attention_dot_o_do": [P, P, P, c_size, c_size, c_size, c_size, S],
     "bf_hip_attention_backward": [P, P, P, P, P, P, P, P, P, P, c_size, c_size, c_size, c_size, c_size, c_float,
                                   c_size, S],

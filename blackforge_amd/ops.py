@@ -548,6 +548,133 @@ def selfAttentionIncrementalBf16(xNew, wq, wk, wv, wout, numHeads: int, cache):
 
 
 # ------------------------------------------------------------------------------------------------
+# a cache with a length per sequence, and drafted tokens (no counterparts in the reference)
+# ------------------------------------------------------------------------------------------------
+def treeVisibility(parents) -> np.ndarray:
+    """Masks for attentionTree from parent indices [..., nodes] (host; a parent comes before its child, a root has a negative
+    one): bit j of a node's mask is set for its ancestors and itself."""
+    parents = np.asarray(parents)
+    _require(parents.shape[-1] <= 64, "treeVisibility: a tree has at most 64 nodes")
+    masks = np.zeros(parents.shape, np.uint64)
+    for at in np.ndindex(parents.shape):
+        parent = int(parents[at])
+        _require(parent < at[-1], f"treeVisibility: node {at[-1]} comes before its parent {parent}")
+        masks[at] = np.uint64(1) << np.uint64(at[-1]) | (masks[at[:-1] + (parent,)] if parent >= 0 else np.uint64(0))
+    return masks
+
+
+def _pointer(t: Optional[DeviceTensor]):
+    return t.ptr if t is not None else None
+
+
+def _check_tree(name, q, kNew, vNew, kCache, vCache, lengths, numHeads, kvHeads, counts, visible):
+    _require(q.rank() == 3 and kNew.rank() == 3 and kCache.rank() == 3, f"{name}: expected [batch, rows, dim] tensors")
+    batch, nodes, dim = q.shape
+    _require(numHeads > 0 and kvHeads > 0 and dim % numHeads == 0 and numHeads % kvHeads == 0, f"{name}: incompatible heads")
+    headDim = dim // numHeads
+    _require(kNew.shape == (batch, nodes, kvHeads * headDim) and vNew.shape == kNew.shape, f"{name}: incompatible new keys and values")
+    _require(kCache.shape == (batch, kCache.shape[1], kvHeads * headDim) and vCache.shape == kCache.shape, f"{name}: incompatible caches")
+    _require(lengths.shape == (batch,) and (counts is None or counts.shape == (batch,)), f"{name}: one length and one count per sequence")
+    _require(visible is None or (visible.shape == (batch, nodes) and visible.itemsize == 8), f"{name}: visible must be 64-bit [batch, nodes]")
+    return batch, nodes, headDim
+
+
+def attentionTree(q, kNew, vNew, kCache, vCache, lengths, numHeads: int, scale: float, counts=None, visible=None,
+                  kvHeads: Optional[int] = None) -> FusedAttentionForwardResult:
+    """Attention of a drafted tree's nodes over a cache (bf_hip_attention_tree); rows past counts[b] are zero."""
+    kvHeads = kvHeads or numHeads
+    batch, nodes, headDim = _check_tree("attentionTree", q, kNew, vNew, kCache, vCache, lengths, numHeads, kvHeads, counts, visible)
+    make = DeviceTensor if counts is None else DeviceTensor.zeros
+    res = FusedAttentionForwardResult(make(q.shape), make((batch, numHeads, nodes)), make((batch, numHeads, nodes)))
+    _call("bf_hip_attention_tree", q.ptr, kNew.ptr, vNew.ptr, kCache.ptr, vCache.ptr, lengths.ptr, _pointer(counts), _pointer(visible),
+          res.output.ptr, res.m.ptr, res.l.ptr, batch, numHeads, kvHeads, nodes, kCache.shape[1], headDim, scale, None)
+    return res
+
+
+def attentionTreeWeights(q, kNew, vNew, kCache, vCache, lengths, numHeads: int, scale: float, weights, counts=None, visible=None,
+                         kvHeads: Optional[int] = None) -> FusedAttentionForwardResult:
+    """attentionTree that adds the weight each row receives to `weights` [batch, groups, capacity], in place."""
+    kvHeads = kvHeads or numHeads
+    batch, nodes, headDim = _check_tree("attentionTreeWeights", q, kNew, vNew, kCache, vCache, lengths, numHeads, kvHeads, counts, visible)
+    capacity = kCache.shape[1]
+    _require(weights.rank() == 3 and weights.shape[0] == batch and weights.shape[2] == capacity, "attentionTreeWeights: weights must be [batch, groups, capacity]")
+    make = DeviceTensor if counts is None else DeviceTensor.zeros
+    res = FusedAttentionForwardResult(make(q.shape), make((batch, numHeads, nodes)), make((batch, numHeads, nodes)))
+    _call("bf_hip_attention_tree_weights", q.ptr, kNew.ptr, vNew.ptr, kCache.ptr, vCache.ptr, lengths.ptr, _pointer(counts), _pointer(visible),
+          res.output.ptr, res.m.ptr, res.l.ptr, weights.ptr, weights.ptr, batch, numHeads, kvHeads, weights.shape[1], nodes, capacity, headDim,
+          scale, None)
+    return res
+
+
+def attentionKeyWeights(q, k, m, l, numHeads: int, scale: float, oldLen: int, groups: int, weights=None, counts=None,
+                        kvHeads: Optional[int] = None) -> DeviceTensor:
+    """The weight each key received in a pass whose statistics are m, l: [batch, groups, rows of k]; added to `weights` if given."""
+    kvHeads = kvHeads or numHeads
+    _require(q.rank() == 3 and k.rank() == 3 and q.shape[0] == k.shape[0], "attentionKeyWeights: expected [batch, rows, dim] tensors")
+    batch, newLen, dim = q.shape
+    _require(numHeads > 0 and dim % numHeads == 0 and k.shape[2] == kvHeads * (dim // numHeads), "attentionKeyWeights: incompatible heads")
+    _require(m.shape == (batch, numHeads, newLen) and l.shape == m.shape, "attentionKeyWeights: statistics must be [batch, heads, newLen]")
+    total = k.shape[1]
+    out = weights if weights is not None else DeviceTensor((batch, groups, total))
+    _require(out.rank() == 3 and out.shape[:2] == (batch, groups) and out.shape[2] >= total, "attentionKeyWeights: weights must be [batch, groups, rows]")
+    _call("bf_hip_attention_key_weights", q.ptr, k.ptr, m.ptr, l.ptr, _pointer(counts), _pointer(weights), out.ptr, batch, numHeads, kvHeads, groups,
+          newLen, total, total, dim // numHeads, scale, oldLen, out.shape[2], None)
+    return out
+
+
+def kvEvict(kCache, vCache, weights, lengths, kvHeads: int, budget: int, recent: int) -> None:
+    """The caches, the weights and the lengths cut down in place to at most `budget` rows (bf_hip_kv_evict)."""
+    _require(kCache.rank() == 3 and vCache.shape == kCache.shape, "kvEvict: expected caches [batch, capacity, dim]")
+    batch, capacity, dim = kCache.shape
+    _require(kvHeads > 0 and dim % kvHeads == 0, "kvEvict: kvHeads must divide dim")
+    _require(weights.rank() == 3 and weights.shape[0] == batch and weights.shape[2] == capacity and lengths.shape == (batch,),
+             "kvEvict: weights must be [batch, groups, capacity], lengths [batch]")
+    _call("bf_hip_kv_evict", kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, None, batch, kvHeads,
+          weights.shape[1], dim // kvHeads, capacity, capacity, budget, recent, None)
+
+
+@dataclass
+class AcceptedPath:
+    path: DeviceTensor      # int32 [batch, nodes], -1 past the path
+    counts: DeviceTensor    # int32 [batch]
+    next: DeviceTensor      # float ids [batch]
+
+
+def treeAccept(logits, tokens, parents, counts=None) -> AcceptedPath:
+    """The path of a drafted tree that greedy choices confirm, and the token after it (bf_hip_tree_accept)."""
+    _require(logits.rank() == 3 and tokens.shape == logits.shape[:2] and parents.shape == tokens.shape,
+             "treeAccept: expected logits [batch, nodes, vocab], tokens and parents [batch, nodes]")
+    batch, nodes, vocab = logits.shape
+    res = AcceptedPath(DeviceTensor((batch, nodes)), DeviceTensor((batch,)), DeviceTensor.zeros((batch,)))
+    _call("bf_hip_tree_accept", logits.ptr, tokens.ptr, parents.ptr, _pointer(counts), res.path.ptr, res.counts.ptr, res.next.ptr, batch, nodes, vocab,
+          None)
+    return res
+
+
+def kvCommit(kCaches, vCaches, kNews, vNews, accepted: AcceptedPath, lengths, weights=None) -> None:
+    """The accepted nodes' keys and values appended to every layer's caches (lists of tensors), the lengths advanced in place."""
+    layers = len(kCaches)
+    _require(layers > 0 and len(vCaches) == layers and len(kNews) == layers and len(vNews) == layers and (weights is None or len(weights) == layers),
+             "kvCommit: one tensor per layer")
+    batch, capacity, dim = kCaches[0].shape
+    nodes = kNews[0].shape[1]
+    for t in list(kCaches) + list(vCaches):
+        _require(t.shape == (batch, capacity, dim), "kvCommit: the layers' caches differ in shape")
+    for t in list(kNews) + list(vNews):
+        _require(t.shape == (batch, nodes, dim), "kvCommit: the new rows must be [batch, nodes, dim]")
+    groups = 1
+    if weights is not None:
+        groups = weights[0].shape[1]
+        for t in weights:
+            _require(t.shape == (batch, groups, capacity), "kvCommit: weights must be [batch, groups, capacity]")
+    _require(accepted.path.shape == (batch, nodes) and accepted.counts.shape == (batch,) and lengths.shape == (batch,),
+             "kvCommit: one path, count and length per sequence")
+    _call("bf_hip_kv_commit", _ptr_array(kCaches), _ptr_array(vCaches), _ptr_array(kNews), _ptr_array(vNews),
+          _ptr_array(weights) if weights is not None else None, layers, accepted.path.ptr, accepted.counts.ptr, lengths.ptr, lengths.ptr, batch, groups,
+          groups, nodes, capacity, dim // groups, None)
+
+
+# ------------------------------------------------------------------------------------------------
 # losses (loss.hpp:20-70)
 # ------------------------------------------------------------------------------------------------
 @dataclass

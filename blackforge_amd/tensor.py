@@ -85,6 +85,19 @@ class DeviceTensor:
         return t
 
     @staticmethod
+    def fromHostInts(host, dtype=np.int32) -> "DeviceTensor":
+        """Device integers (lengths, counts, node indices: int32; masks of tree nodes: uint64)."""
+        host = np.ascontiguousarray(host, dtype=dtype)
+        t = DeviceTensor(host.shape, host.itemsize)
+        capi.call("bf_hip_memcpy_h2d", t.ptr, host.ctypes.data_as(ctypes.c_void_p), t._bytes)
+        return t
+
+    def toHostInts(self) -> np.ndarray:
+        out = np.empty(self.shape, np.int32 if self.itemsize == 4 else np.uint64)
+        capi.call("bf_hip_memcpy_d2h", out.ctypes.data_as(ctypes.c_void_p), self.ptr, self._bytes)
+        return out
+
+    @staticmethod
     def zeros(shape: Sequence[int]) -> "DeviceTensor":
         t = DeviceTensor(shape)
         capi.call("bf_hip_fill_zero", t.ptr, t._bytes, None)

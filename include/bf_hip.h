@@ -463,6 +463,71 @@ int bf_hip_attention_forward_rows_indirect(const float* q, const float* k, const
 int bf_hip_argmax_last_position_device(const float* logits, size_t seq, size_t vocab, float* token, float* history, size_t historyLen,
                                        int* position, int advance, long long historyOffset, bf_stream_t stream);
 int bf_hip_counter_add(int* counter, int by, bf_stream_t stream);
+/* ---- A cache with a length per sequence, and drafted tokens (no counterparts in the reference, whose generation loop
+ * decodes one token at a time and drops no cached position, main.cpp:594-617).
+ * kCache, vCache: [batch, capacity, kvHeads * headDim], of which the first lengths[b] rows of sequence b are in use (the
+ * layout of hip::KVCache); lengths, counts and the like are int32 in DEVICE memory, one per sequence, so that a host may
+ * launch ahead of the device; kernels hold them inside what the tensors have room for.  Query head h reads key head
+ * h * kvHeads / heads (kvHeads must divide heads); headDim <= 256, at most 64 new tokens ("nodes") a sequence.
+ *
+ * attention_tree: the new tokens are the nodes of a drafted tree; their keys and values, kNew and vNew [batch, nodes,
+ * kvHeads * headDim], are not yet in the cache.  Node i of sequence b sees the cached rows j < lengths[b] and the new rows
+ * j < counts[b] whose bit j is set in visible[b, i] (its ancestors and, normally, itself).  counts NULL: all nodes.
+ * visible NULL: bits 0..i, i.e. a chain; one node is an ordinary decoding step.  q, out: [batch, nodes, heads * headDim]; m, l:
+ * [batch, heads, nodes], the statistics of attention_forward (maximum of the scaled scores and sum of exp(score - m)),
+ * each may be NULL.  A node that sees nothing, or nothing but scores of -infinity, gets out = 0, l = 0 (m = -infinity).
+ * Nodes i >= counts[b] are neither read nor written, and neither are rows that a node does not see: what lies there may
+ * be NaN.  Any alignment; 16-byte aligned operands with headDim a multiple of 4 are faster. */
+int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
+                          const int* counts, const uint64_t* visible, float* out, float* m, float* l, size_t batch, size_t heads, size_t kvHeads,
+                          size_t nodes, size_t capacity, size_t headDim, float scale, bf_stream_t stream);
+/* attention_tree that also keeps account of the attention weight (the probabilities exp(score - m) / l) that each row
+ * receives, summed over the nodes and the query heads of a group: head h belongs to group h * groups / heads, groups must
+ * divide kvHeads.  weights: [batch, groups, capacity].  For j < lengths[b] weightsOut[b, g, j] = weightsIn[b, g, j] + the
+ * weight received; the new rows' weights follow at j = lengths[b] + node (where the row will be once it is appended) as far
+ * as the capacity goes, without weightsIn; entries past them stay as they were.  weightsIn may be NULL (zeros) or be
+ * weightsOut itself. */
+int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
+                                  const int* counts, const uint64_t* visible, float* out, float* m, float* l, const float* weightsIn,
+                                  float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t nodes, size_t capacity,
+                                  size_t headDim, float scale, bf_stream_t stream);
+/* The same account for a pass that has already run, a prompt's above all: from the statistics m, l [batch, heads, newLen]
+ * that attention_forward left for q [batch, newLen, heads * headDim] and the keys k [batch, kvRows, kvHeads * headDim],
+ * weightsOut[b, g, j] = weightsIn[b, g, j] + sum over the heads of group g and the queries i < counts[b] (NULL: newLen)
+ * with j <= oldLen + i of exp(score_ij - m_i) / l_i, for j < totalLen; weights: [batch, groups, weightRows].  A row with
+ * l = 0 gives nothing.  weightsIn may be NULL (zeros) or weightsOut itself.  oldLen >= totalLen - 1: no causal mask. */
+int bf_hip_attention_key_weights(const float* q, const float* k, const float* m, const float* l, const int* counts, const float* weightsIn,
+                                 float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t newLen, size_t totalLen,
+                                 size_t kvRows, size_t headDim, float scale, size_t oldLen, size_t weightRows, bf_stream_t stream);
+/* A cache cut down to `budget` rows a sequence: of each group of heads the last `recent` rows stay and, of those before,
+ * the budget - recent with the largest weights (equal weights: the lower row; a NaN counts as -infinity), in their order;
+ * a sequence of at most `budget` rows keeps all.  weights: [batch, groups, capacity] as above, group g owning the key heads
+ * g * kvHeads / groups ..; with one group whole rows stay or go.  Rows, values and weights go to kOut, vOut [batch,
+ * outCapacity, kvHeads * headDim] and weightsOut [batch, groups, outCapacity] (budget <= outCapacity); what lies past the
+ * rows that remain is left as it was.  kOut, vOut and weightsOut may be kCache, vCache and weights themselves, all three
+ * together (outCapacity = capacity then).  lengthsOut (may be NULL, may be lengths) receives min(lengths, budget); kept
+ * [batch, groups, budget] (may be NULL) the kept rows' old places.  Layers that share `lengths`: pass lengthsOut = NULL
+ * for all but the last. */
+int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weights, const int* lengths, float* kOut, float* vOut, float* weightsOut,
+                    int* lengthsOut, int* kept, size_t batch, size_t kvHeads, size_t groups, size_t headDim, size_t capacity, size_t outCapacity,
+                    size_t budget, size_t recent, bf_stream_t stream);
+/* Which path of a drafted tree the model itself would have taken: node 0, the last token that is certain, and from each
+ * accepted node the lowest-numbered child (parents[b, j] = the node, j past it) whose token is the first maximum of the
+ * node's logits [batch, nodes, vocab].  tokens: float ids [batch, nodes]; parents [batch, nodes], each before its child
+ * (a root's own parent is ignored); counts NULL: all nodes.  path [batch, nodes] receives the accepted nodes and then -1,
+ * pathCounts[b] their number (0 if counts[b] is 0), next[b] the token chosen after the last of them, as a float id.  A
+ * NaN is never chosen unless it is element 0 (argmax_last_position's rule).  vocab <= 2^24. */
+int bf_hip_tree_accept(const float* logits, const float* tokens, const int* parents, const int* counts, int* path, int* pathCounts, float* next,
+                       size_t batch, size_t nodes, size_t vocab, bf_stream_t stream);
+/* The accepted nodes' keys and values appended to the caches of all layers: row path[b, i] of kNew, vNew (of every layer,
+ * [batch, nodes, kvHeads * headDim]) to row lengths[b] + i, i < pathCounts[b]; lengthsOut (may be NULL, may be lengths)
+ * receives lengths + pathCounts.  The arrays of pointers are HOST arrays of `layers` entries.  weights (NULL, or a tensor
+ * per layer) [batch, groups, capacity]: the weight at lengths[b] + path[b, i] moves to lengths[b] + i.  path is [batch, nodes].
+ * A sequence whose path does not fit (an entry that is no node, a count past `nodes`, no room in the cache) is left as it
+ * was, its length too. */
+int bf_hip_kv_commit(float* const* kCaches, float* const* vCaches, const float* const* kNew, const float* const* vNew, float* const* weights,
+                     size_t layers, const int* path, const int* pathCounts, const int* lengths, int* lengthsOut, size_t batch, size_t kvHeads,
+                     size_t groups, size_t nodes, size_t capacity, size_t headDim, bf_stream_t stream);
 /* computeDKernel: fused_attention.cu:166-190   D[b,h,i] = dot(out[b,i,h,:], dOut[b,i,h,:]) */
 int bf_hip_attention_dot_o_do(const float* out, const float* dOut, float* D, size_t batch, size_t heads,
                               size_t newLen, size_t dim, bf_stream_t stream);
