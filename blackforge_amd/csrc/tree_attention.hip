@@ -7,7 +7,9 @@
 // Query head h reads key head h * kvHeads / heads.
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <initializer_list>
 
 namespace bf {
 namespace {
@@ -33,48 +35,464 @@ __device__ __forceinline__ unsigned long long newRowsSeen(const TreeParams& p, i
     return bits & upTo;
 }
 
-// One wavefront per (sequence, head, node), a key at a time.
-__global__ void __launch_bounds__(256) treeAttentionKernel(TreeParams p) {
+// ---- the pass over the cache -------------------------------------------------------------------
+// The rows of one key head, all its queries of all nodes (row = node * share + head within the share), times the cache is a
+// pair of matrix products with a softmax between them, and the cache is read once: 8 bytes of keys and values against four
+// flops a row; fp32 matrix instructions (v_mfma_f32_16x16x4_f32) keep up with the memory up to about 32 rows.
+//
+// A wavefront holds RT tiles of 16 rows (the queries as B operands, the output as accumulators) and takes 16 keys at a
+// time: S^T = K Q^T leaves a lane with 4 keys of one row, which is already the B operand of O^T += V^T P^T, so neither
+// scores nor probabilities leave their registers.  Keys and values go from memory straight into A operands, 16 bytes a
+// lane and no LDS: a dot product does not care about the order of its terms, nor do the rows of O^T, so lane (i, g) of
+// 16 x 4 loads head columns 16 s + 4 g .. of key i, and columns 4 i .. of the values of keys 4 g ...  The loads of the
+// next keys are issued as soon as the products have read the registers of these.
+//
+// Softmax about a reference that moves only when a score outgrows it by 2^8 (common for the first keys, then rare), so a
+// tile normally needs no maximum across lanes and no rescaling.  d = c dot - ref in one fused operation, c = scale log2(e):
+// the error of d is relative to d, not to the score.  The true maximum is kept beside it for the statistics.
+struct TilePlan {
+    int target;          // chunks per (key head, group of row tiles) that the launch wants in total over the sequences
+    int minChunk;        // keys a chunk has at least
+    int items;           // workgroups along the sequences' chunks: at least the number of chunks there will be
+    int rowGroups;       // groups of RT row tiles
+    float4v* partStat;   // [item][kvHeads][rows]: ref, l, largest dot product
+    float* partOut;      // [item][kvHeads][rows][hd], relative to ref
+    int2* span;          // [batch]: first item and number of items of a sequence
+    float* scores;       // [batch][kvHeads][rows][scorePitch] dot products with the cached rows (NULL: not kept)
+    float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
+    float2* stat2;       // [batch][kvHeads][rows]: ref and 1 / l of the whole row, for the account of the weights
+    int scorePitch;
+    float c;             // |scale| log2(e)
+};
+
+// Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for
+// each.  Returns this item's sequence (-1: there is none) and its chunk.
+struct Chunk { int b, first, count, start, end; };
+__device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& plan, int item) {
     const int lane = threadIdx.x & 63;
-    const size_t row = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= size_t(p.batch) * p.heads * p.nodes) return;
-    const int i = int(row % p.nodes), h = int(row / p.nodes % p.heads), b = int(row / p.nodes / p.heads);
-    const int length = rowsInUse(p, b), count = nodesInUse(p, b);
-    if (i >= count) return;
-    const int kvDim = p.kvHeads * p.hd, kh = h / (p.heads / p.kvHeads);
-    const unsigned long long seen = newRowsSeen(p, b, i, count);
-    const float* q = p.q + (size_t(b) * p.nodes + i) * p.heads * p.hd + size_t(h) * p.hd;
-    float qr[4], acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    long long total = 0;   // in units of 64 rows
+    for (int b0 = 0; b0 < p.batch; b0 += 64) total += b0 + lane < p.batch ? (rowsInUse(p, b0 + lane) + 63) / 64 : 0;
+    if (p.batch > 1) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) qr[u] = lane + 64 * u < p.hd ? q[lane + 64 * u] : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int j = 0; j < length + count; ++j) {
-        const bool fresh = j >= length;
-        if (fresh && !(seen >> (j - length) & 1)) continue;
-        const size_t at = (fresh ? size_t(b) * p.nodes + (j - length) : size_t(b) * p.capacity + j) * kvDim + size_t(kh) * p.hd;
-        const float* kr = (fresh ? p.kNew : p.k) + at;
-        const float* vr = (fresh ? p.vNew : p.v) + at;
-        float dot = 0.0f;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (lane + 64 * u < p.hd) dot += qr[u] * kr[lane + 64 * u];
-        const float s = waveSum(dot) * p.scale;
-        const float mm = fmaxf(m, s);
-        const float keep = m == -INFINITY ? 0.0f : expf(m - mm), w = s == -INFINITY ? 0.0f : expf(s - mm);
-        l = l * keep + w;
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (lane + 64 * u < p.hd) acc[u] = acc[u] * keep + w * vr[lane + 64 * u];
-        m = mm;
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+    } else {
+        total = __shfl(total, 0, 64);
     }
-    float* out = p.out + (size_t(b) * p.nodes + i) * p.heads * p.hd + size_t(h) * p.hd;
+    const int even = int(min((total + plan.target - 1) / plan.target, (long long)(1 << 24)));
+    const int size = max(plan.minChunk, even * 64);
+    Chunk c{-1, 0, 0, 0, 0};
+    int before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+        const int length = b0 + lane < p.batch ? rowsInUse(p, b0 + lane) : 0;
+        const int mine = b0 + lane < p.batch ? max(1, (length + size - 1) / size) : 0;
+        int upTo = mine;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (lane + 64 * u < p.hd) out[lane + 64 * u] = l == 0.0f ? 0.0f : acc[u] / l;
-    if (lane == 0) {
-        const size_t stat = (size_t(b) * p.heads + h) * p.nodes + i;
-        p.m[stat] = m;
-        p.l[stat] = l;
+        for (int off = 1; off < 64; off <<= 1) {
+            const int o = __shfl_up(upTo, off, 64);
+            if (lane >= off) upTo += o;
+        }
+        const unsigned long long past = __ballot(before + upTo > item);
+        if (past != 0) {
+            const int at = __ffsll(past) - 1;
+            c.b = __builtin_amdgcn_readfirstlane(b0 + at);
+            c.count = __builtin_amdgcn_readlane(mine, at);
+            c.first = before + __builtin_amdgcn_readlane(upTo, at) - c.count;
+            const int len = __builtin_amdgcn_readlane(length, at);
+            c.start = (item - c.first) * size;
+            c.end = min(c.start + size, len);
+            return c;
+        }
+        before += __builtin_amdgcn_readlane(upTo, 63);
+    }
+    return c;
+}
+
+// MODE 2: headDim == HDP, 16-byte aligned; 1: a multiple of 4, aligned; 0: anything
+template <int MODE, int W>
+__device__ __forceinline__ void loadColumns(float (&x)[W], const float* row, int d, int hd) {
+    if constexpr (MODE == 0) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[j] = d + j < hd ? row[d + j] : 0.0f;
+    } else {
+        const bool in = MODE == 2 || d < hd;
+        const float* at = row + (in ? d : 0);
+        if constexpr (W == 4) {
+            const float4v f = loadf4(at);
+            x[0] = in ? f.x : 0.0f; x[1] = in ? f.y : 0.0f; x[2] = in ? f.z : 0.0f; x[3] = in ? f.w : 0.0f;
+        } else {
+            const float2v f = *reinterpret_cast<const float2v*>(at);
+            x[0] = in ? f.x : 0.0f; x[1] = in ? f.y : 0.0f;
+        }
+    }
+}
+
+// A row's statistics from its reference, the sum about it and its largest dot product
+__device__ __forceinline__ void finishStats(const TreeParams& p, const TilePlan& plan, int b, int kh, int row, float ref, float sum, float top) {
+    const int share = p.heads / p.kvHeads;
+    const size_t stat = (size_t(b) * p.heads + kh * share + row % share) * p.nodes + row / share;
+    const bool empty = sum == 0.0f;
+    if (p.m) p.m[stat] = empty ? -INFINITY : top * fabsf(p.scale);
+    if (p.l) p.l[stat] = empty ? 0.0f : sum * __builtin_amdgcn_exp2f(-fmaf(top, plan.c, -ref));
+    if (plan.stat2) plan.stat2[(size_t(b) * p.kvHeads + kh) * p.nodes * share + row] = make_float2(ref, empty ? 0.0f : 1.0f / sum);
+}
+
+constexpr float kNoRef = -3.402823466e38f;   // a reference below every score: the first real one moves it
+constexpr float kRefSlack = 8.0f;
+
+// wavefronts per SIMD that the registers of a form allow
+constexpr int tileWaves(int hdp, int rt) { return hdp * rt <= 64 ? 3 : hdp * rt <= 256 && hdp <= 128 ? 2 : 1; }
+template <int HDP, int RT, int MODE>
+__global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeParams p, TilePlan plan) {
+    constexpr int KS = HDP / 16;                    // 16-column steps of the dot products
+    constexpr int VW = HDP >= 64 ? 4 : 2;           // value columns a lane loads at once
+    constexpr int VU = HDP / (16 * VW);             // such loads
+    extern __shared__ float smem[];
+    __shared__ float4v sStat[4][RT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+    // the row groups of one chunk next to each other on one XCD (workgroups go to the 8 XCDs in turn), where they share its reads
+    const unsigned perXcd = blockIdx.x / 8, flat = perXcd / plan.rowGroups * 8 + blockIdx.x % 8;
+    const int rowGroup = perXcd % plan.rowGroups;
+    const int kh = flat % p.kvHeads, item = flat / p.kvHeads;
+    if (item >= plan.items) return;
+    const Chunk ch = findChunk(p, plan, item);
+    if (ch.b < 0) return;
+    const int b = ch.b, share = p.heads / p.kvHeads, rows = p.nodes * share, hd = p.hd;
+    const int count = nodesInUse(p, b), live = count * share;     // rows past `live` belong to no node
+    if (item == ch.first && kh == 0 && rowGroup == 0 && threadIdx.x == 0) plan.span[b] = make_int2(ch.first, ch.count);
+    const int row0 = rowGroup * RT * 16;
+    if (row0 >= live) return;
+    const int tiles = min(RT, (live - row0 + 15) / 16);
+    const size_t kvDim = size_t(p.kvHeads) * hd;
+    const float* kb = p.k + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
+    const float* vb = p.v + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
+
+    float q[RT][KS][4];
+    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const int row = row0 + t * 16 + i16;
+        const bool on = row < live;
+        const int node = on ? row / share : 0, h = kh * share + (on ? row % share : 0);
+        const float* src = p.q + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            loadColumns<MODE, 4>(q[t][s], src, 16 * s + 4 * g, hd);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[t][s][c] = on ? q[t][s][c] * sign : 0.0f;
+        }
+    }
+    float4v o[RT][VU][VW];
+    float ref[RT], l[RT], top[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        ref[t] = kNoRef; l[t] = 0.0f; top[t] = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int w = 0; w < VW; ++w) o[t][u][w] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    float k[KS][4], v[VU][4][VW];
+    // key i16 of 16 from `row`; `last`: the last row that may be read
+    auto loadK = [&](const float* base, int row, int last) {
+        const float* src = base + size_t(min(row + i16, last)) * kvDim;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(k[s], src, 16 * s + 4 * g, hd);
+    };
+    auto loadV = [&](const float* base, int row, int last) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float* src = base + size_t(min(row + 4 * g + r, last)) * kvDim;
+#pragma unroll
+            for (int u = 0; u < VU; ++u) loadColumns<MODE, VW>(v[u][r], src, u * 16 * VW + i16 * VW, hd);
+        }
+    };
+    auto dotProducts = [&](int t) {
+        float4v even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;   // two chains: half the error, and none waits for the one before
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][0], q[t][s][0], even, 0, 0, 0);
+            odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][1], q[t][s][1], odd, 0, 0, 0);
+            even = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][2], q[t][s][2], even, 0, 0, 0);
+            odd = __builtin_amdgcn_mfma_f32_16x16x4f32(k[s][3], q[t][s][3], odd, 0, 0, 0);
+        }
+        return even + odd;
+    };
+    // dot products to probabilities about ref[t] (-infinity: not seen)
+    auto probabilities = [&](int t, float (&x)[4]) {
+        float d[4];
+        bool over = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            top[t] = fmaxf(top[t], x[r]);
+            d[r] = fmaf(x[r], plan.c, -ref[t]);
+            over = over || d[r] > kRefSlack;
+        }
+        if (__any(over)) {
+            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float moved = mx == -INFINITY ? ref[t] : fmaxf(ref[t], mx * plan.c);
+            const float keep = __builtin_amdgcn_exp2f(ref[t] - moved);
+            ref[t] = moved;
+            l[t] *= keep;
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) o[t][u][w] = o[t][u][w] * keep;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[r] = fmaf(x[r], plan.c, -moved);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_exp2f(d[r]);
+        l[t] += (x[0] + x[1]) + (x[2] + x[3]);
+    };
+    auto addValues = [&](int t, const float (&x)[4]) {
+#pragma unroll
+        for (int u = 0; u < VU; ++u)
+#pragma unroll
+            for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[t][u][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u][r][w], x[r], o[t][u][w], 0, 0, 0);
+    };
+
+    // cached rows: the four wavefronts take 16 keys in turn
+    int key = ch.start + wave * 16;
+    if (key < ch.end) {
+        const int last = ch.end - 1;
+        loadK(kb, key, last);
+        loadV(vb, key, last);
+        for (; key < ch.end; key += 64) {
+            const bool whole = key + 16 <= ch.end;
+            float x[RT][4];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                if (t < tiles) {
+                    const float4v dots = dotProducts(t);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[t][r] = whole || key + 4 * g + r < ch.end ? dots[r] : -INFINITY;
+                }
+            }
+            if (key + 64 < ch.end) loadK(kb, key + 64, last);
+            if (plan.scores) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t) {
+                    const int row = row0 + t * 16 + i16;
+                    if (row < live) storef4(plan.scores + ((size_t(b) * p.kvHeads + kh) * rows + row) * plan.scorePitch + key + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
+                }
+            }
+            if (!whole) {   // values of keys past the end: whatever lies there must not meet a weight of zero
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+#pragma unroll
+                    for (int u = 0; u < VU; ++u)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) v[u][r][w] = key + 4 * g + r < ch.end ? v[u][r][w] : 0.0f;
+            }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                if (t < tiles) {
+                    probabilities(t, x[t]);
+                    addValues(t, x[t]);
+                }
+            }
+            if (key + 64 < ch.end) loadV(vb, key + 64, last);
+        }
+    }
+    // new rows: with the sequence's last chunk, the wavefronts again taking 16 in turn
+    if (item == ch.first + ch.count - 1 && wave * 16 < count) {
+        const int j0 = wave * 16;
+        const float* kn = p.kNew + size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
+        const float* vn = p.vNew + size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
+        loadK(kn, j0, count - 1);
+        loadV(vn, j0, count - 1);
+        // values that are not finite must reach the rows that see them and no others: they are taken out of the products
+        unsigned odd = 0;   // bit r: this lane holds one of key 4 g + r
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    if (j0 + 4 * g + r >= count) v[u][r][w] = 0.0f;
+                    if (!(fabsf(v[u][r][w]) < INFINITY)) { odd |= 1u << r; v[u][r][w] = 0.0f; }
+                }
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if (t < tiles) {
+                const int row = row0 + t * 16 + i16;
+                const unsigned long long seen = row < live ? newRowsSeen(p, b, row / share, count) >> j0 >> (4 * g) : 0ull;
+                const float4v dots = dotProducts(t);
+                float x[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = seen >> r & 1 ? dots[r] : -INFINITY;
+                if (plan.newScores && row < live)
+                    storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[0], x[1], x[2], x[3]});
+                probabilities(t, x);
+                addValues(t, x);
+                for (int r = 0; r < 4; ++r) {
+                    unsigned long long holders = __ballot(odd >> r & 1);
+                    while (holders != 0) {
+                        const int group = (__ffsll(holders) - 1) >> 4;
+                        holders &= ~(0xFFFFull << (16 * group));
+                        const float weight = __shfl(x[r], group * 16 + i16, 64);
+                        const bool sees = __shfl(int(seen >> r & 1), group * 16 + i16, 64) != 0;
+                        const float* src = vn + size_t(j0 + 4 * group + r) * kvDim;
+#pragma unroll
+                        for (int u = 0; u < VU; ++u)
+#pragma unroll
+                            for (int w = 0; w < VW; ++w)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int d = u * 16 * VW + (4 * g + e) * VW + w;
+                                    const float value = d < hd ? src[d] : 0.0f;
+                                    if (sees && !(fabsf(value) < INFINITY)) o[t][u][w][e] += weight * value;
+                                }
+                    }
+                }
+            }
+        }
+    }
+
+    // the four wavefronts' states joined through LDS, [wave][row][HDP + 4]
+    constexpr int PITCH = HDP + 4;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        if (t < tiles) {
+            float sum = l[t], mx = top[t];
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (g == 0) sStat[wave][t * 16 + i16] = float4v{ref[t], sum, mx, 0.0f};
+            float* mine = smem + (wave * RT * 16 + t * 16 + i16) * PITCH;
+#pragma unroll
+            for (int u = 0; u < VU; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) mine[u * 16 * VW + (4 * g + e) * VW + w] = o[t][u][w][e];
+        }
+    }
+    __syncthreads();
+    const bool only = ch.count == 1;
+    const int liveHere = min(live - row0, tiles * 16);
+    // sixteen threads a row, four columns at a time
+    for (int e = threadIdx.x; e < liveHere * 16; e += 256) {
+        const int r = e >> 4, part = e & 15, row = row0 + r;
+        float4v st[4];
+        float most = kNoRef, mx = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            st[w] = sStat[w][r];
+            most = fmaxf(most, st[w].x);
+            mx = fmaxf(mx, st[w].z);
+        }
+        float f[4], sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            f[w] = __builtin_amdgcn_exp2f(st[w].x - most);
+            sum += st[w].y * f[w];
+        }
+        const int node = row / share, h = kh * share + row % share;
+        const float inv = only ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
+        float* dst = only ? p.out + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd
+                          : plan.partOut + ((size_t(item) * p.kvHeads + kh) * rows + row) * hd;
+        for (int d = part * 4; d < hd; d += 64) {
+            float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) acc = acc + *reinterpret_cast<const float4v*>(smem + (w * RT * 16 + r) * PITCH + d) * f[w];
+            acc = acc * inv;
+            if (MODE != 0) {
+                storef4(dst + d, acc);
+            } else {
+                for (int j = 0; j < 4; ++j)
+                    if (d + j < hd) dst[d + j] = acc[j];
+            }
+        }
+        if (part == 0) {
+            if (only) finishStats(p, plan, b, kh, row, most, sum, mx);
+            else plan.partStat[(size_t(item) * p.kvHeads + kh) * rows + row] = float4v{most, sum, mx, 0.0f};
+        }
+    }
+}
+
+// The chunks of a row put together: a wavefront per (sequence, key head, row), lanes over the head's columns.
+__global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan plan) {
+    const int lane = threadIdx.x & 63, share = p.heads / p.kvHeads, rows = p.nodes * share;
+    const size_t flat = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (flat >= size_t(p.batch) * p.kvHeads * rows) return;
+    const int row = int(flat % rows), kh = int(flat / rows % p.kvHeads), b = int(flat / rows / p.kvHeads);
+    if (row >= nodesInUse(p, b) * share) return;
+    const int2 span = plan.span[b];
+    if (span.y == 1) return;   // written by its only chunk
+    const size_t step = size_t(p.kvHeads) * rows, at = size_t(span.x) * step + size_t(kh) * rows + row;
+    float most = kNoRef, mx = -INFINITY, sum = 0.0f;
+    for (int c = lane; c < span.y; c += 64) {
+        const float4v st = plan.partStat[at + c * step];
+        const float to = fmaxf(most, st.x);
+        sum = sum * __builtin_amdgcn_exp2f(most - to) + st.y * __builtin_amdgcn_exp2f(st.x - to);
+        most = to;
+        mx = fmaxf(mx, st.z);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float other = __shfl_xor(most, off, 64), otherSum = __shfl_xor(sum, off, 64), to = fmaxf(most, other);
+        sum = sum * __builtin_amdgcn_exp2f(most - to) + otherSum * __builtin_amdgcn_exp2f(other - to);
+        most = to;
+        mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    }
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int c = 0; c < span.y; ++c) {
+        const float f = __builtin_amdgcn_exp2f(plan.partStat[at + c * step].x - most);
+        const float* src = plan.partOut + (at + c * step) * p.hd;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (lane + 64 * j < p.hd) acc[j] += f * src[lane + 64 * j];
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float* dst = p.out + (size_t(b) * p.nodes + row / share) * p.heads * p.hd + size_t(kh * share + row % share) * p.hd;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (lane + 64 * j < p.hd) dst[lane + 64 * j] = acc[j] * inv;
+    if (lane == 0) finishStats(p, plan, b, kh, row, most, sum, mx);
+}
+
+// The weights from the kept dot products: four keys a thread, the rows of a group one after the other.  The new rows' weights
+// are made by the first workgroup of each (sequence, group).
+__global__ void __launch_bounds__(256) treeWeightsFromScoresKernel(TreeParams p, TilePlan plan) {
+    const int g = blockIdx.y, b = blockIdx.z, share = p.heads / p.kvHeads, rows = p.nodes * share;
+    const int length = rowsInUse(p, b), count = nodesInUse(p, b), live = count * share;
+    const int perGroup = p.kvHeads / p.groups, kh0 = g * perGroup;
+    const size_t at = (size_t(b) * p.groups + g) * p.capacity;
+    const int j = (int(blockIdx.x) * 256 + int(threadIdx.x)) * 4;
+    if (j < length) {
+        float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int kh = kh0; kh < kh0 + perGroup; ++kh) {
+            const size_t first = (size_t(b) * p.kvHeads + kh) * rows;
+#pragma unroll 4
+            for (int row = 0; row < live; ++row) {
+                const float2 st = plan.stat2[first + row];
+                const float4v x = loadf4(plan.scores + (first + row) * plan.scorePitch + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < length) p.weightsOut[at + j + e] = (p.weightsIn ? p.weightsIn[at + j + e] : 0.0f) + sum[e];
+    }
+    if (blockIdx.x == 0 && threadIdx.x < unsigned(count) && length + int(threadIdx.x) < p.capacity) {
+        float sum = 0.0f;
+        for (int kh = kh0; kh < kh0 + perGroup; ++kh) {
+            const size_t first = (size_t(b) * p.kvHeads + kh) * rows;
+            for (int row = 0; row < live; ++row) {
+                const float2 st = plan.stat2[first + row];
+                sum += __builtin_amdgcn_exp2f(fmaf(plan.newScores[(first + row) * 64 + threadIdx.x], plan.c, -st.x)) * st.y;
+            }
+        }
+        p.weightsOut[at + length + threadIdx.x] = sum;
     }
 }
 
@@ -136,6 +554,39 @@ __global__ void __launch_bounds__(256) keyWeightsKernel(KeyWeightParams p) {
     if (lane == 0) p.weightsOut[at] = (p.weightsIn ? p.weightsIn[at] : 0.0f) + sum;
 }
 
+template <int HDP, int RT, int MODE>
+int launchTilesOf(const TreeParams& p, const TilePlan& plan, unsigned grid, hipStream_t s) {
+    constexpr size_t smem = size_t(4) * RT * 16 * (HDP + 4) * sizeof(float);
+    const int st = allowDynamicSharedMemory(reinterpret_cast<const void*>(treeTilesKernel<HDP, RT, MODE>), smem);
+    if (st != BF_OK) return st;
+    treeTilesKernel<HDP, RT, MODE><<<grid, 256, smem, s>>>(p, plan);
+    BF_LAUNCH_CHECK();
+    return BF_OK;
+}
+template <int HDP, int RT>
+int launchTilesMode(const TreeParams& p, const TilePlan& plan, int mode, unsigned grid, hipStream_t s) {
+    if (mode == 2) return launchTilesOf<HDP, RT, 2>(p, plan, grid, s);
+    if (mode == 1) return launchTilesOf<HDP, RT, 1>(p, plan, grid, s);
+    return launchTilesOf<HDP, RT, 0>(p, plan, grid, s);
+}
+template <int HDP>
+int launchTilesRows(const TreeParams& p, const TilePlan& plan, int rt, int mode, unsigned grid, hipStream_t s) {
+    if constexpr (HDP <= 128) {
+        if (rt == 4) return launchTilesMode<HDP, 4>(p, plan, mode, grid, s);
+        if (rt == 2) return launchTilesMode<HDP, 2>(p, plan, mode, grid, s);
+    }
+    return launchTilesMode<HDP, 1>(p, plan, mode, grid, s);
+}
+int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int mode, unsigned grid, hipStream_t s) {
+    switch (hdp) {
+        case 32: return launchTilesRows<32>(p, plan, rt, mode, grid, s);
+        case 64: return launchTilesRows<64>(p, plan, rt, mode, grid, s);
+        case 128: return launchTilesRows<128>(p, plan, rt, mode, grid, s);
+        case 192: return launchTilesRows<192>(p, plan, rt, mode, grid, s);
+        default: return launchTilesRows<256>(p, plan, rt, mode, grid, s);
+    }
+}
+
 int checkHeads(const char* fn, size_t heads, size_t kvHeads, size_t groups, size_t headDim) {
     if (heads == 0 || kvHeads == 0 || heads % kvHeads != 0)
         return failInvalid(fn, "kvHeads (" + std::to_string(kvHeads) + ") must divide the number of heads (" + std::to_string(heads) + ")");
@@ -158,14 +609,61 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.nodes = int(nodes);
     p.capacity = int(capacity); p.hd = int(headDim);
     hipStream_t s = asStream(stream);
-    const size_t stats = batch * heads * nodes;
-    Scratch own(p.m && p.l ? 0 : 2 * stats * sizeof(float));
+    const size_t share = heads / kvHeads, rows = nodes * share;
+    const bool keepScores = weights && capacity != 0 && rows <= 16;
+    const bool recompute = weights && capacity != 0 && !keepScores;
+    // Row tiles a wavefront holds: what the rows fill, up to the registers there are
+    const int hdp = headDim <= 32 ? 32 : headDim <= 64 ? 64 : headDim <= 128 ? 128 : headDim <= 192 ? 192 : 256;
+    const int most = hdp <= 128 ? 4 : 1;
+    const int rt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
+    TilePlan plan{};
+    plan.rowGroups = int((rows + 16 * rt - 1) / (16 * rt));
+    plan.minChunk = 128;
+    plan.target = int(std::max<size_t>(1, size_t(computeUnits()) * 4 / (kvHeads * size_t(plan.rowGroups))));
+    const size_t chunksAtMost = batch * std::max<size_t>(1, (capacity + plan.minChunk - 1) / plan.minChunk);
+    plan.items = int(std::min(chunksAtMost, size_t(plan.target) + batch));
+    plan.c = float(std::fabs(double(p.scale)) * 1.4426950408889634074);
+    plan.scorePitch = int((capacity + 15) / 16 * 16);
+    const bool join = size_t(plan.items) > batch;
+    const size_t slots = size_t(plan.items) * kvHeads * rows, rowsAll = batch * kvHeads * rows;
+    const size_t need[] = {join ? slots * sizeof(float4v) : 0, join ? slots * headDim * sizeof(float) : 0, batch * sizeof(int2),
+                           keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, keepScores ? rowsAll * 64 * sizeof(float) : 0,
+                           weights ? rowsAll * sizeof(float2) : 0, recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
+    size_t bytes = 0, offset[7];
+    for (int i = 0; i < 7; ++i) {
+        offset[i] = bytes;
+        bytes += (need[i] + 255) / 256 * 256;
+    }
+    Scratch own(bytes);
     if (own.status != BF_OK) return own.status;
-    if (!p.m) p.m = own.as<float>();
-    if (!p.l) p.l = own.as<float>() + stats;
-    treeAttentionKernel<<<unsigned((stats + 3) / 4), 256, 0, s>>>(p);
-    BF_LAUNCH_CHECK();
-    if (weights && capacity != 0) {
+    auto part = [&](int i) { return need[i] != 0 ? own.as<char>() + offset[i] : nullptr; };
+    plan.partStat = reinterpret_cast<float4v*>(part(0));
+    plan.partOut = reinterpret_cast<float*>(part(1));
+    plan.span = reinterpret_cast<int2*>(part(2));
+    plan.scores = reinterpret_cast<float*>(part(3));
+    plan.newScores = reinterpret_cast<float*>(part(4));
+    plan.stat2 = reinterpret_cast<float2*>(part(5));
+    if (float* own2 = reinterpret_cast<float*>(part(6))) {
+        if (!p.m) p.m = own2;
+        if (!p.l) p.l = own2 + rowsAll;
+    }
+    const unsigned grid = unsigned((size_t(plan.items) * kvHeads + 7) / 8 * 8 * size_t(plan.rowGroups));
+    auto aligned = [](std::initializer_list<const void*> ptrs) {
+        uintptr_t bits = 0;
+        for (const void* x : ptrs) bits |= reinterpret_cast<uintptr_t>(x);
+        return (bits & 15u) == 0;
+    };
+    const int mode = headDim % 4 != 0 || !aligned({p.q, p.kNew, p.vNew, p.k, p.v, p.out}) ? 0 : headDim == size_t(hdp) ? 2 : 1;
+    st = launchTiles(p, plan, hdp, rt, mode, grid, s);
+    if (st != BF_OK) return st;
+    if (join) {
+        treeJoinKernel<<<unsigned((rowsAll + 3) / 4), 256, 0, s>>>(p, plan);
+        BF_LAUNCH_CHECK();
+    }
+    if (keepScores) {
+        treeWeightsFromScoresKernel<<<dim3(unsigned((capacity + 1023) / 1024), unsigned(groups), unsigned(batch)), 256, 0, s>>>(p, plan);
+        BF_LAUNCH_CHECK();
+    } else if (recompute) {
         treeWeightsKernel<<<unsigned((batch * groups * capacity + 3) / 4), 256, 0, s>>>(p);
         BF_LAUNCH_CHECK();
     }
