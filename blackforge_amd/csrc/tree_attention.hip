@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(256) treeWeightsFromScoresKernel(TreeParams p,
     const int perGroup = p.kvHeads / p.groups, kh0 = g * perGroup;
     const size_t at = (size_t(b) * p.groups + g) * p.capacity;
     const int j = (int(blockIdx.x) * 256 + int(threadIdx.x)) * 4;
-    if (j < length) {
+    if (plan.scores && j < length) {
         float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
         for (int kh = kh0; kh < kh0 + perGroup; ++kh) {
             const size_t first = (size_t(b) * p.kvHeads + kh) * rows;
@@ -496,62 +496,179 @@ __global__ void __launch_bounds__(256) treeWeightsFromScoresKernel(TreeParams p,
     }
 }
 
-// One wavefront per (sequence, group, row of the cache): the row's weight from the statistics of the pass above.
-__global__ void __launch_bounds__(256) treeWeightsKernel(TreeParams p) {
-    const int lane = threadIdx.x & 63;
-    const size_t row = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= size_t(p.batch) * p.groups * p.capacity) return;
-    const int j = int(row % p.capacity), g = int(row / p.capacity % p.groups), b = int(row / p.capacity / p.groups);
-    const int length = rowsInUse(p, b), count = nodesInUse(p, b);
-    if (j >= length + count) return;
-    const bool fresh = j >= length;
-    const int kvDim = p.kvHeads * p.hd, share = p.heads / p.kvHeads, perGroup = p.heads / p.groups;
-    const float* rows = fresh ? p.kNew + (size_t(b) * p.nodes + (j - length)) * kvDim : p.k + (size_t(b) * p.capacity + j) * kvDim;
-    float sum = 0.0f;
-    for (int h = g * perGroup; h < (g + 1) * perGroup; ++h) {
-        const float* kr = rows + size_t(h / share) * p.hd;
-        for (int i = 0; i < count; ++i) {
-            if (fresh && !(newRowsSeen(p, b, i, count) >> (j - length) & 1)) continue;
-            const float* q = p.q + (size_t(b) * p.nodes + i) * p.heads * p.hd + size_t(h) * p.hd;
-            float dot = 0.0f;
-            for (int d = lane; d < p.hd; d += 64) dot += q[d] * kr[d];
-            const float s = waveSum(dot) * p.scale;
-            const size_t stat = (size_t(b) * p.heads + h) * p.nodes + i;
-            if (p.l[stat] > 0.0f) sum += expf(s - p.m[stat]) / p.l[stat];
-        }
-    }
-    if (lane == 0) p.weightsOut[row] = (!fresh && p.weightsIn ? p.weightsIn[row] : 0.0f) + sum;
-}
-
+// ---- the weight of keys from statistics --------------------------------------------------------
 struct KeyWeightParams {
     const float* q; const float* k; const float* m; const float* l;
-    const int* counts; const float* weightsIn; float* weightsOut;
+    const int* counts;     // queries of each sequence that count (NULL: all)
+    const int* lengths;    // keys of each sequence that are in use (NULL: totalLen)
+    const float* weightsIn; float* weightsOut;
+    float* part;           // [batch][heads][queryChunks][totalLen] sums over a chunk of queries
     int batch, heads, kvHeads, groups, newLen, totalLen, kvRows, hd, oldLen, weightRows;
+    int keyBlocks, queryChunk, queryChunks;
     float scale;
 };
 
-// One wavefront per (sequence, group, key).
-__global__ void __launch_bounds__(256) keyWeightsKernel(KeyWeightParams p) {
-    const int lane = threadIdx.x & 63;
-    const size_t row = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (row >= size_t(p.batch) * p.groups * p.totalLen) return;
-    const int j = int(row % p.totalLen), g = int(row / p.totalLen % p.groups), b = int(row / p.totalLen / p.groups);
-    const int count = p.counts ? min(max(p.counts[b], 0), p.newLen) : p.newLen;
-    const int share = p.heads / p.kvHeads, perGroup = p.heads / p.groups;
+// What sequence b has in use
+__device__ __forceinline__ int queriesOf(const KeyWeightParams& p, int b) { return p.counts ? min(max(p.counts[b], 0), p.newLen) : p.newLen; }
+__device__ __forceinline__ int keysOf(const KeyWeightParams& p, int b) { return p.lengths ? min(max(p.lengths[b], 0), p.totalLen) : p.totalLen; }
+// Queries of chunk c that see a key of a block starting at `key`: [from, to), empty if from >= to
+__device__ __forceinline__ int2 queriesOfChunk(const KeyWeightParams& p, int queries, int c, int key) {
+    return make_int2(max(c * p.queryChunk, (key - p.oldLen) & ~15), min((c + 1) * p.queryChunk, queries));
+}
+
+// sum_i exp(s_ij - m_i) / l_i with the keys' owner as the workgroup: a wavefront holds KT tiles of 16 keys as B operands and
+// walks the queries 16 at a time, S = Q K^T leaving a lane with 4 queries of one key, whose probabilities it adds up; no
+// lane needs another's until the end.  Bound by the matrix instruction (2 headDim flops a pair, the prompt read from L2).
+// The four wavefronts of a workgroup take neighbouring keys and the same queries.
+template <int HDP, int KT, int MODE>
+__global__ void __launch_bounds__(256, 2) keyWeightTilesKernel(KeyWeightParams p) {
+    constexpr int KS = HDP / 16;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+    // chunks of queries outermost and the blocks of keys with the most queries (the lowest) first
+    const size_t pairs = size_t(p.batch) * p.heads;
+    const size_t flat = blockIdx.x;
+    const int h = int(flat % pairs % p.heads), b = int(flat % pairs / p.heads);
+    const int block = int(flat / pairs) % p.keyBlocks, chunk = int(flat / pairs) / p.keyBlocks;
+    const int keys = keysOf(p, b), key0 = block * KT * 64, mine = key0 + wave * KT * 16;
+    const int2 span = queriesOfChunk(p, queriesOf(p, b), chunk, key0);
+    if (mine >= keys || span.x >= span.y) return;
+    const int hd = p.hd, kh = h / (p.heads / p.kvHeads);
+    const size_t kvDim = size_t(p.kvHeads) * hd, dim = size_t(p.heads) * hd;
+    float k[KT][KS][4];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const float* src = p.k + (size_t(b) * p.kvRows + min(mine + t * 16 + i16, keys - 1)) * kvDim + size_t(kh) * hd;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(k[t][s], src, 16 * s + 4 * g, hd);
+    }
+    const float* qb = p.q + size_t(b) * p.newLen * dim + size_t(h) * hd;
+    const float* mb = p.m + (size_t(b) * p.heads + h) * p.newLen;
+    const float* lb = p.l + (size_t(b) * p.heads + h) * p.newLen;
+    float q[KS][4], m[4], l[4], sum[KT] = {};
+    auto load = [&](int i) {
+        const float* src = qb + size_t(min(i + i16, span.y - 1)) * dim;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(q[s], src, 16 * s + 4 * g, hd);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = min(i + 4 * g + r, span.y - 1);
+            m[r] = mb[row];
+            l[r] = lb[row];
+        }
+    };
+    // queries below `mine - oldLen` see none of this wavefront's keys
+    int i = max(span.x, (mine - p.oldLen) & ~15);
+    if (i < span.y) load(i);
+    for (; i < span.y; i += 16) {
+        const bool whole = i + 16 <= span.y && mine + KT * 16 - 1 <= p.oldLen + i;   // every pair seen
+        float4v dots[KT];
+        float top[4], over[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            over[r] = l[r] > 0.0f ? __builtin_amdgcn_rcpf(l[r]) : 0.0f;
+            top[r] = l[r] > 0.0f ? m[r] : INFINITY;      // a row that saw nothing gives nothing
+        }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            float4v even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                even = __builtin_amdgcn_mfma_f32_16x16x4f32(q[s][0], k[t][s][0], even, 0, 0, 0);
+                odd = __builtin_amdgcn_mfma_f32_16x16x4f32(q[s][1], k[t][s][1], odd, 0, 0, 0);
+                even = __builtin_amdgcn_mfma_f32_16x16x4f32(q[s][2], k[t][s][2], even, 0, 0, 0);
+                odd = __builtin_amdgcn_mfma_f32_16x16x4f32(q[s][3], k[t][s][3], odd, 0, 0, 0);
+            }
+            dots[t] = even + odd;
+        }
+        if (i + 16 < span.y) load(i + 16);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            float w[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f((dots[t][r] * p.scale - top[r]) * kLog2e) * over[r];
+            if (!whole) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = i + 4 * g + r;
+                    w[r] = row < span.y && mine + t * 16 + i16 <= p.oldLen + row ? w[r] : 0.0f;
+                }
+            }
+            sum[t] += (w[0] + w[1]) + (w[2] + w[3]);
+        }
+    }
+    float* dst = p.part + ((size_t(b) * p.heads + h) * p.queryChunks + chunk) * p.totalLen;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        sum[t] += __shfl_xor(sum[t], 16, 64);
+        sum[t] += __shfl_xor(sum[t], 32, 64);
+        const int key = mine + t * 16 + i16;
+        if (g == 0 && key < keys) dst[key] = sum[t];
+    }
+}
+
+// The sums of a group's heads and of the chunks of queries added up, in order.
+__global__ void __launch_bounds__(256) keyWeightJoinKernel(KeyWeightParams p, int keysPerBlock) {
+    const int j = int(blockIdx.x) * 256 + int(threadIdx.x), g = blockIdx.y, b = blockIdx.z;
+    if (j >= keysOf(p, b)) return;
+    const int queries = queriesOf(p, b), perGroup = p.heads / p.groups, key0 = j / keysPerBlock * keysPerBlock;
     float sum = 0.0f;
     for (int h = g * perGroup; h < (g + 1) * perGroup; ++h) {
-        const float* kr = p.k + (size_t(b) * p.kvRows + j) * p.kvHeads * p.hd + size_t(h / share) * p.hd;
-        for (int i = max(0, j - p.oldLen); i < count; ++i) {
-            const float* q = p.q + (size_t(b) * p.newLen + i) * p.heads * p.hd + size_t(h) * p.hd;
-            float dot = 0.0f;
-            for (int d = lane; d < p.hd; d += 64) dot += q[d] * kr[d];
-            const float s = waveSum(dot) * p.scale;
-            const size_t stat = (size_t(b) * p.heads + h) * p.newLen + i;
-            if (p.l[stat] > 0.0f) sum += expf(s - p.m[stat]) / p.l[stat];
+        const float* src = p.part + (size_t(b) * p.heads + h) * p.queryChunks * p.totalLen + j;
+        for (int c = 0; c < p.queryChunks; ++c) {
+            const int2 span = queriesOfChunk(p, queries, c, key0);
+            if (span.x < span.y) sum += src[size_t(c) * p.totalLen];
         }
     }
     const size_t at = (size_t(b) * p.groups + g) * p.weightRows + j;
-    if (lane == 0) p.weightsOut[at] = (p.weightsIn ? p.weightsIn[at] : 0.0f) + sum;
+    p.weightsOut[at] = (p.weightsIn ? p.weightsIn[at] : 0.0f) + sum;
+}
+
+// ---- launches ----------------------------------------------------------------------------------
+bool aligned16(std::initializer_list<const void*> ptrs) {
+    uintptr_t bits = 0;
+    for (const void* x : ptrs) bits |= reinterpret_cast<uintptr_t>(x);
+    return (bits & 15u) == 0;
+}
+int paddedHeadDim(size_t hd) { return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : hd <= 192 ? 192 : 256; }
+
+template <int HDP, int KT>
+int launchKeyTiles(const KeyWeightParams& p, int mode, size_t grid, hipStream_t s) {
+    if (mode == 2) keyWeightTilesKernel<HDP, KT, 2><<<unsigned(grid), 256, 0, s>>>(p);
+    else if (mode == 1) keyWeightTilesKernel<HDP, KT, 1><<<unsigned(grid), 256, 0, s>>>(p);
+    else keyWeightTilesKernel<HDP, KT, 0><<<unsigned(grid), 256, 0, s>>>(p);
+    BF_LAUNCH_CHECK();
+    return BF_OK;
+}
+
+int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
+    const int hdp = paddedHeadDim(size_t(p.hd)), keysPerBlock = (hdp <= 128 ? 4 : 2) * 64;
+    p.keyBlocks = (p.totalLen + keysPerBlock - 1) / keysPerBlock;
+    const size_t pairs = size_t(p.batch) * p.heads, blocks = pairs * p.keyBlocks;
+    // Queries a workgroup walks: as many as leave four workgroups a compute unit, so that the sums it leaves behind are few
+    int chunk = 2048;
+    while (chunk > 128 && blocks * size_t((p.newLen + chunk - 1) / chunk) < size_t(computeUnits()) * 4) chunk /= 2;
+    p.queryChunk = chunk;
+    p.queryChunks = std::max(1, (p.newLen + chunk - 1) / chunk);
+    const size_t grid = blocks * p.queryChunks;
+    if (grid >= (size_t(1) << 31)) return failInvalid(fn, "shape too large");
+    Scratch part(pairs * p.queryChunks * p.totalLen * sizeof(float));
+    if (part.status != BF_OK) return part.status;
+    p.part = part.as<float>();
+    if (p.newLen > 0) {
+        const int mode = p.hd % 4 != 0 || !aligned16({p.q, p.k}) ? 0 : p.hd == hdp ? 2 : 1;
+        int st = BF_OK;
+        switch (hdp) {
+            case 32: st = launchKeyTiles<32, 4>(p, mode, grid, s); break;
+            case 64: st = launchKeyTiles<64, 4>(p, mode, grid, s); break;
+            case 128: st = launchKeyTiles<128, 4>(p, mode, grid, s); break;
+            case 192: st = launchKeyTiles<192, 2>(p, mode, grid, s); break;
+            default: st = launchKeyTiles<256, 2>(p, mode, grid, s); break;
+        }
+        if (st != BF_OK) return st;
+    }
+    keyWeightJoinKernel<<<dim3(unsigned((p.totalLen + 255) / 256), unsigned(p.groups), unsigned(p.batch)), 256, 0, s>>>(p, keysPerBlock);
+    BF_LAUNCH_CHECK();
+    return BF_OK;
 }
 
 template <int HDP, int RT, int MODE>
@@ -613,7 +730,7 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const bool keepScores = weights && capacity != 0 && rows <= 16;
     const bool recompute = weights && capacity != 0 && !keepScores;
     // Row tiles a wavefront holds: what the rows fill, up to the registers there are
-    const int hdp = headDim <= 32 ? 32 : headDim <= 64 ? 64 : headDim <= 128 ? 128 : headDim <= 192 ? 192 : 256;
+    const int hdp = paddedHeadDim(headDim);
     const int most = hdp <= 128 ? 4 : 1;
     const int rt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
     TilePlan plan{};
@@ -627,7 +744,7 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const bool join = size_t(plan.items) > batch;
     const size_t slots = size_t(plan.items) * kvHeads * rows, rowsAll = batch * kvHeads * rows;
     const size_t need[] = {join ? slots * sizeof(float4v) : 0, join ? slots * headDim * sizeof(float) : 0, batch * sizeof(int2),
-                           keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, keepScores ? rowsAll * 64 * sizeof(float) : 0,
+                           keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, weights ? rowsAll * 64 * sizeof(float) : 0,
                            weights ? rowsAll * sizeof(float2) : 0, recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
     size_t bytes = 0, offset[7];
     for (int i = 0; i < 7; ++i) {
@@ -648,24 +765,24 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
         if (!p.l) p.l = own2 + rowsAll;
     }
     const unsigned grid = unsigned((size_t(plan.items) * kvHeads + 7) / 8 * 8 * size_t(plan.rowGroups));
-    auto aligned = [](std::initializer_list<const void*> ptrs) {
-        uintptr_t bits = 0;
-        for (const void* x : ptrs) bits |= reinterpret_cast<uintptr_t>(x);
-        return (bits & 15u) == 0;
-    };
-    const int mode = headDim % 4 != 0 || !aligned({p.q, p.kNew, p.vNew, p.k, p.v, p.out}) ? 0 : headDim == size_t(hdp) ? 2 : 1;
+    const int mode = headDim % 4 != 0 || !aligned16({p.q, p.kNew, p.vNew, p.k, p.v, p.out}) ? 0 : headDim == size_t(hdp) ? 2 : 1;
     st = launchTiles(p, plan, hdp, rt, mode, grid, s);
     if (st != BF_OK) return st;
     if (join) {
         treeJoinKernel<<<unsigned((rowsAll + 3) / 4), 256, 0, s>>>(p, plan);
         BF_LAUNCH_CHECK();
     }
-    if (keepScores) {
-        treeWeightsFromScoresKernel<<<dim3(unsigned((capacity + 1023) / 1024), unsigned(groups), unsigned(batch)), 256, 0, s>>>(p, plan);
+    if (weights && capacity != 0) {
+        // the new rows' weights, and the cached rows' where their dot products were kept
+        treeWeightsFromScoresKernel<<<dim3(keepScores ? unsigned((capacity + 1023) / 1024) : 1u, unsigned(groups), unsigned(batch)), 256, 0, s>>>(p, plan);
         BF_LAUNCH_CHECK();
-    } else if (recompute) {
-        treeWeightsKernel<<<unsigned((batch * groups * capacity + 3) / 4), 256, 0, s>>>(p);
-        BF_LAUNCH_CHECK();
+    }
+    if (recompute) {
+        KeyWeightParams w{};
+        w.q = p.q; w.k = p.k; w.m = p.m; w.l = p.l; w.counts = p.counts; w.lengths = p.lengths; w.weightsIn = p.weightsIn; w.weightsOut = p.weightsOut;
+        w.batch = p.batch; w.heads = p.heads; w.kvHeads = p.kvHeads; w.groups = p.groups; w.newLen = p.nodes; w.totalLen = p.capacity;
+        w.kvRows = p.capacity; w.hd = p.hd; w.oldLen = p.capacity; w.weightRows = p.capacity; w.scale = p.scale;
+        return keyWeights(fn, w, s);
     }
     return BF_OK;
 }
@@ -713,9 +830,7 @@ int bf_hip_attention_key_weights(const float* q, const float* k, const float* m,
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.newLen = headDim == 0 ? 0 : int(newLen);
     p.totalLen = int(totalLen); p.kvRows = int(kvRows); p.hd = int(headDim); p.oldLen = int(oldLen); p.weightRows = int(weightRows);
     p.scale = scale;
-    keyWeightsKernel<<<unsigned((batch * groups * totalLen + 3) / 4), 256, 0, asStream(stream)>>>(p);
-    BF_LAUNCH_CHECK();
-    return BF_OK;
+    return keyWeights(__func__, p, asStream(stream));
 }
 
 }  // extern "C"
