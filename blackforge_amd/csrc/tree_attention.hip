@@ -606,6 +606,162 @@ __global__ void __launch_bounds__(256, 2) keyWeightTilesKernel(KeyWeightParams p
     }
 }
 
+// The same with every fp32 product as six bf16 ones (v_mfma_f32_16x16x32_bf16), for passes of many queries, which are
+// bound by the matrix instruction: an fp32 value is the exact sum of three bf16 terms, x = h + m + l, and h h', h m', m h',
+// h l', l h', m m' hold everything above 2^-24 of the product, at 6/16 of the fp32 instruction's time.  h h' and the rest
+// are two accumulators, so that the small terms are added among themselves first.
+//
+// The keys' terms stay in registers; 32 queries at a time are split once for the four wavefronts and handed over through
+// LDS (two buffers, one barrier a step, the next step's rows in flight in registers meanwhile), their maxima and reciprocal
+// sums beside them.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+struct Terms { bf16x8 t[3]; };
+__device__ __forceinline__ Terms splitTerms(const float (&x)[8]) {
+    Terms out;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const __bf16 h = static_cast<__bf16>(x[j]);
+        const float r1 = x[j] - static_cast<float>(h);
+        const __bf16 m = static_cast<__bf16>(r1);
+        out.t[0][j] = h;
+        out.t[1][j] = m;
+        out.t[2][j] = static_cast<__bf16>(r1 - static_cast<float>(m));
+    }
+    return out;
+}
+template <int HDP, int KT, int MODE>
+__global__ void __launch_bounds__(256, 2) keyWeightSplitKernel(KeyWeightParams p) {
+    constexpr int ST = HDP / 32, PITCH = HDP + 8, ROWS = 32, CHUNKS = ROWS * HDP / 8, PER = (CHUNKS + 255) / 256;
+    __shared__ __attribute__((aligned(16))) __bf16 sQ[2][3][ROWS][PITCH];
+    __shared__ __attribute__((aligned(16))) float sTop[2][ROWS], sOver[2][ROWS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+    const size_t pairs = size_t(p.batch) * p.heads;
+    const size_t flat = blockIdx.x;
+    const int h = int(flat % pairs % p.heads), b = int(flat % pairs / p.heads);
+    const int block = int(flat / pairs) % p.keyBlocks, chunk = int(flat / pairs) / p.keyBlocks;
+    const int keys = keysOf(p, b), key0 = block * KT * 64, mine = key0 + wave * KT * 16;
+    const int2 span = queriesOfChunk(p, queriesOf(p, b), chunk, key0);
+    if (key0 >= keys || span.x >= span.y) return;
+    const int hd = p.hd, kh = h / (p.heads / p.kvHeads);
+    const size_t kvDim = size_t(p.kvHeads) * hd, dim = size_t(p.heads) * hd;
+    Terms k[KT][ST];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const float* src = p.k + (size_t(b) * p.kvRows + min(mine + t * 16 + i16, keys - 1)) * kvDim + size_t(kh) * hd;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            float x[2][4], y[8];
+            loadColumns<MODE, 4>(x[0], src, 32 * s + 8 * g, hd);
+            loadColumns<MODE, 4>(x[1], src, 32 * s + 8 * g + 4, hd);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j / 4][j % 4];
+            k[t][s] = splitTerms(y);
+        }
+    }
+    const float* qb = p.q + size_t(b) * p.newLen * dim + size_t(h) * hd;
+    const float* mb = p.m + (size_t(b) * p.heads + h) * p.newLen;
+    const float* lb = p.l + (size_t(b) * p.heads + h) * p.newLen;
+    float q[PER][2][4], m = 0.0f, l = 0.0f, sum[KT] = {};
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int e = int(threadIdx.x) + 256 * u, row = e / (HDP / 8), col = e % (HDP / 8) * 8;
+            if (CHUNKS % 256 == 0 || e < CHUNKS) {
+                const float* src = qb + size_t(min(i0 + row, span.y - 1)) * dim;
+                loadColumns<MODE, 4>(q[u][0], src, col, hd);
+                loadColumns<MODE, 4>(q[u][1], src, col + 4, hd);
+            }
+        }
+        if (threadIdx.x < ROWS) {
+            const int row = min(i0 + int(threadIdx.x), span.y - 1);
+            m = mb[row];
+            l = lb[row];
+        }
+    };
+    auto stage = [&](int buf) {
+#pragma unroll
+        for (int u = 0; u < PER; ++u) {
+            const int e = int(threadIdx.x) + 256 * u, row = e / (HDP / 8), col = e % (HDP / 8) * 8;
+            if (CHUNKS % 256 == 0 || e < CHUNKS) {
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = q[u][j / 4][j % 4];
+                const Terms t = splitTerms(y);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) *reinterpret_cast<bf16x8*>(&sQ[buf][x][row][col]) = t.t[x];
+            }
+        }
+        if (threadIdx.x < ROWS) {
+            sTop[buf][threadIdx.x] = l > 0.0f ? m : INFINITY;      // a row that saw nothing gives nothing
+            sOver[buf][threadIdx.x] = l > 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
+        }
+    };
+    load(span.x);
+    stage(0);
+    __syncthreads();
+    int buf = 0;
+    for (int i0 = span.x; i0 < span.y; i0 += ROWS, buf ^= 1) {
+        const bool more = i0 + ROWS < span.y;
+        if (more) load(i0 + ROWS);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int i = i0 + half * 16;
+            // none of these queries counts, or sees one of this wavefront's keys
+            if (mine >= keys || i >= span.y || i + 15 + p.oldLen < mine) continue;
+            const bool whole = i + 16 <= span.y && mine + KT * 16 - 1 <= p.oldLen + i;
+            float4v large[KT], small[KT];
+#pragma unroll
+            for (int t = 0; t < KT; ++t) large[t] = small[t] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < ST; ++s) {
+                bf16x8 a[3];
+#pragma unroll
+                for (int x = 0; x < 3; ++x) a[x] = *reinterpret_cast<const bf16x8*>(&sQ[buf][x][half * 16 + i16][32 * s + 8 * g]);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) {
+                    small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[2], k[t][s].t[0], small[t], 0, 0, 0);
+                    large[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], k[t][s].t[0], large[t], 0, 0, 0);
+                }
+#pragma unroll
+                for (int t = 0; t < KT; ++t) small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], k[t][s].t[2], small[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], k[t][s].t[1], small[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[1], k[t][s].t[0], small[t], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[0], k[t][s].t[1], small[t], 0, 0, 0);
+            }
+            const float4v top = *reinterpret_cast<const float4v*>(&sTop[buf][half * 16 + 4 * g]);
+            const float4v over = *reinterpret_cast<const float4v*>(&sOver[buf][half * 16 + 4 * g]);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const float4v dots = large[t] + small[t];
+                float w[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) w[r] = __builtin_amdgcn_exp2f(fmaf(dots[r], p.scale, -top[r]) * kLog2e) * over[r];
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = i + 4 * g + r;
+                        w[r] = row < span.y && mine + t * 16 + i16 <= p.oldLen + row ? w[r] : 0.0f;
+                    }
+                }
+                sum[t] += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+        }
+        if (more) stage(buf ^ 1);
+        __syncthreads();
+    }
+    float* dst = p.part + ((size_t(b) * p.heads + h) * p.queryChunks + chunk) * p.totalLen;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        sum[t] += __shfl_xor(sum[t], 16, 64);
+        sum[t] += __shfl_xor(sum[t], 32, 64);
+        const int key = mine + t * 16 + i16;
+        if (g == 0 && key < keys) dst[key] = sum[t];
+    }
+}
+
 // The sums of a group's heads and of the chunks of queries added up, in order.
 __global__ void __launch_bounds__(256) keyWeightJoinKernel(KeyWeightParams p, int keysPerBlock) {
     const int j = int(blockIdx.x) * 256 + int(threadIdx.x), g = blockIdx.y, b = blockIdx.z;
@@ -640,8 +796,20 @@ int launchKeyTiles(const KeyWeightParams& p, int mode, size_t grid, hipStream_t 
     return BF_OK;
 }
 
+template <int HDP, int KT>
+int launchKeySplit(const KeyWeightParams& p, int mode, size_t grid, hipStream_t s) {
+    if (mode == 2) keyWeightSplitKernel<HDP, KT, 2><<<unsigned(grid), 256, 0, s>>>(p);
+    else if (mode == 1) keyWeightSplitKernel<HDP, KT, 1><<<unsigned(grid), 256, 0, s>>>(p);
+    else keyWeightSplitKernel<HDP, KT, 0><<<unsigned(grid), 256, 0, s>>>(p);
+    BF_LAUNCH_CHECK();
+    return BF_OK;
+}
+
 int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
-    const int hdp = paddedHeadDim(size_t(p.hd)), keysPerBlock = (hdp <= 128 ? 4 : 2) * 64;
+    const int hdp = paddedHeadDim(size_t(p.hd));
+    // many queries: bound by the products, which the bf16 route does faster; few: by reading the keys
+    const bool split = hdp <= 128 && p.newLen > 64;
+    const int keysPerBlock = (hdp > 128 || (split && hdp == 128) ? 2 : 4) * 64;
     p.keyBlocks = (p.totalLen + keysPerBlock - 1) / keysPerBlock;
     const size_t pairs = size_t(p.batch) * p.heads, blocks = pairs * p.keyBlocks;
     // Queries a workgroup walks: as many as leave four workgroups a compute unit, so that the sums it leaves behind are few
@@ -657,7 +825,9 @@ int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
     if (p.newLen > 0) {
         const int mode = p.hd % 4 != 0 || !aligned16({p.q, p.k}) ? 0 : p.hd == hdp ? 2 : 1;
         int st = BF_OK;
-        switch (hdp) {
+        if (split) {
+            st = hdp == 32 ? launchKeySplit<32, 4>(p, mode, grid, s) : hdp == 64 ? launchKeySplit<64, 4>(p, mode, grid, s) : launchKeySplit<128, 2>(p, mode, grid, s);
+        } else switch (hdp) {
             case 32: st = launchKeyTiles<32, 4>(p, mode, grid, s); break;
             case 64: st = launchKeyTiles<64, 4>(p, mode, grid, s); break;
             case 128: st = launchKeyTiles<128, 4>(p, mode, grid, s); break;
