@@ -9,7 +9,9 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
+#include <type_traits>
 
 namespace bf {
 namespace {
@@ -56,12 +58,12 @@ struct TilePlan {
     int items;           // workgroups along the sequences' chunks: at least the number of chunks there will be
     int rowGroups;       // groups of RT row tiles
     float4v* partStat;   // [item][kvHeads][rows]: ref, l, largest dot product
-    float* partOut;      // [item][kvHeads][rows][hd], relative to ref
+    float* partOut;      // [item][kvHeads][rows][partPitch], relative to ref
     int2* span;          // [batch]: first item and number of items of a sequence
     float* scores;       // [batch][kvHeads][rows][scorePitch] dot products with the cached rows (NULL: not kept)
     float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
     float2* stat2;       // [batch][kvHeads][rows]: ref and 1 / l of the whole row, for the account of the weights
-    int scorePitch;
+    int scorePitch, partPitch;
     float c;             // |scale| log2(e)
 };
 
@@ -141,7 +143,7 @@ constexpr float kRefSlack = 8.0f;
 
 // wavefronts per SIMD that the registers of a form allow
 constexpr int tileWaves(int hdp, int rt) { return hdp * rt <= 64 ? 3 : hdp * rt <= 256 && hdp <= 128 ? 2 : 1; }
-template <int HDP, int RT, int MODE>
+template <int HDP, int RT, int MODE, bool SCORES>
 __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeParams p, TilePlan plan) {
     constexpr int KS = HDP / 16;                    // 16-column steps of the dot products
     constexpr int VW = HDP >= 64 ? 4 : 2;           // value columns a lane loads at once
@@ -218,86 +220,100 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         }
         return even + odd;
     };
-    // dot products to probabilities about ref[t] (-infinity: not seen)
-    auto probabilities = [&](int t, float (&x)[4]) {
-        float d[4];
-        bool over = false;
+    // dot products of N tiles to probabilities about ref (-infinity: not seen)
+    auto probabilities = [&](auto tileCount, float (&x)[RT][4]) {
+        constexpr int N = decltype(tileCount)::value;
+        float d[N][4];
+        float most = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            top[t] = fmaxf(top[t], x[r]);
-            d[r] = fmaf(x[r], plan.c, -ref[t]);
-            over = over || d[r] > kRefSlack;
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) d[t][r] = fmaf(x[t][r], plan.c, -ref[t]);
+            top[t] = fmaxf(top[t], fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+            most = fmaxf(most, fmaxf(fmaxf(d[t][0], d[t][1]), fmaxf(d[t][2], d[t][3])));
         }
-        if (__any(over)) {
-            float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float moved = mx == -INFINITY ? ref[t] : fmaxf(ref[t], mx * plan.c);
-            const float keep = __builtin_amdgcn_exp2f(ref[t] - moved);
-            ref[t] = moved;
-            l[t] *= keep;
+        if (__any(most > kRefSlack)) {
 #pragma unroll
-            for (int u = 0; u < VU; ++u)
+            for (int t = 0; t < N; ++t) {
+                float mx = fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3]));
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float moved = mx == -INFINITY ? ref[t] : fmaxf(ref[t], mx * plan.c);
+                const float keep = __builtin_amdgcn_exp2f(ref[t] - moved);
+                ref[t] = moved;
+                l[t] *= keep;
 #pragma unroll
-                for (int w = 0; w < VW; ++w) o[t][u][w] = o[t][u][w] * keep;
+                for (int u = 0; u < VU; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) d[r] = fmaf(x[r], plan.c, -moved);
+                    for (int w = 0; w < VW; ++w) o[t][u][w] = o[t][u][w] * keep;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) d[t][r] = fmaf(x[t][r], plan.c, -moved);
+            }
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = __builtin_amdgcn_exp2f(d[r]);
-        l[t] += (x[0] + x[1]) + (x[2] + x[3]);
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) x[t][r] = __builtin_amdgcn_exp2f(d[t][r]);
+            l[t] += (x[t][0] + x[t][1]) + (x[t][2] + x[t][3]);
+        }
     };
     auto addValues = [&](int t, const float (&x)[4]) {
 #pragma unroll
-        for (int u = 0; u < VU; ++u)
+        for (int r = 0; r < 4; ++r)       // products of one key after another's: none waits for the accumulator of the one before
 #pragma unroll
-            for (int w = 0; w < VW; ++w)
+            for (int u = 0; u < VU; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[t][u][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u][r][w], x[r], o[t][u][w], 0, 0, 0);
+                for (int w = 0; w < VW; ++w) o[t][u][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u][r][w], x[r], o[t][u][w], 0, 0, 0);
     };
 
-    // cached rows: the four wavefronts take 16 keys in turn
-    int key = ch.start + wave * 16;
-    if (key < ch.end) {
+    // Cached rows: the four wavefronts take 16 keys in turn.  The body is straight-line code for the number of row tiles in
+    // use, and no load in it stands behind a branch (the waits for the loads before it would have to assume the worst).
+    auto walk = [&](auto tileCount) {
+        constexpr int N = decltype(tileCount)::value;
         const int last = ch.end - 1;
+        int key = ch.start + wave * 16;
+        if (key >= ch.end) return;
         loadK(kb, key, last);
         loadV(vb, key, last);
         for (; key < ch.end; key += 64) {
-            const bool whole = key + 16 <= ch.end;
             float x[RT][4];
 #pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if (t < tiles) {
-                    const float4v dots = dotProducts(t);
+            for (int t = 0; t < N; ++t) {
+                const float4v dots = dotProducts(t);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) x[t][r] = whole || key + 4 * g + r < ch.end ? dots[r] : -INFINITY;
+                for (int r = 0; r < 4; ++r) x[t][r] = dots[r];
+            }
+            loadK(kb, key + 64, last);   // past the end: the last row again
+            if (key + 16 > ch.end) {     // values of keys past the end: whatever lies there must not meet a weight of zero
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool in = key + 4 * g + r < ch.end;
+#pragma unroll
+                    for (int t = 0; t < N; ++t) x[t][r] = in ? x[t][r] : -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < VU; ++u)
+#pragma unroll
+                        for (int w = 0; w < VW; ++w) v[u][r][w] = in ? v[u][r][w] : 0.0f;
                 }
             }
-            if (key + 64 < ch.end) loadK(kb, key + 64, last);
-            if (plan.scores) {
+            if constexpr (SCORES) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
+                for (int t = 0; t < N; ++t) {
                     const int row = row0 + t * 16 + i16;
                     if (row < live) storef4(plan.scores + ((size_t(b) * p.kvHeads + kh) * rows + row) * plan.scorePitch + key + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
                 }
             }
-            if (!whole) {   // values of keys past the end: whatever lies there must not meet a weight of zero
+            probabilities(tileCount, x);
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-#pragma unroll
-                    for (int u = 0; u < VU; ++u)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w) v[u][r][w] = key + 4 * g + r < ch.end ? v[u][r][w] : 0.0f;
-            }
-#pragma unroll
-            for (int t = 0; t < RT; ++t) {
-                if (t < tiles) {
-                    probabilities(t, x[t]);
-                    addValues(t, x[t]);
-                }
-            }
-            if (key + 64 < ch.end) loadV(vb, key + 64, last);
+            for (int t = 0; t < N; ++t) addValues(t, x[t]);
+            loadV(vb, key + 64, last);
         }
+    };
+    if (tiles == RT) walk(std::integral_constant<int, RT>{});
+    if constexpr (RT >= 2) { if (tiles == 1) walk(std::integral_constant<int, 1>{}); }
+    if constexpr (RT >= 4) {
+        if (tiles == 2) walk(std::integral_constant<int, 2>{});
+        if (tiles == 3) walk(std::integral_constant<int, 3>{});
     }
     // new rows: with the sequence's last chunk, the wavefronts again taking 16 in turn
     if (item == ch.first + ch.count - 1 && wave * 16 < count) {
@@ -317,38 +333,40 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
                     if (j0 + 4 * g + r >= count) v[u][r][w] = 0.0f;
                     if (!(fabsf(v[u][r][w]) < INFINITY)) { odd |= 1u << r; v[u][r][w] = 0.0f; }
                 }
+        float x[RT][4];
+        unsigned long long seen[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            if (t < tiles) {
-                const int row = row0 + t * 16 + i16;
-                const unsigned long long seen = row < live ? newRowsSeen(p, b, row / share, count) >> j0 >> (4 * g) : 0ull;
-                const float4v dots = dotProducts(t);
-                float x[4];
+            const int row = row0 + t * 16 + i16;
+            seen[t] = row < live ? newRowsSeen(p, b, row / share, count) >> j0 >> (4 * g) : 0ull;
+            const float4v dots = dotProducts(t);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = seen >> r & 1 ? dots[r] : -INFINITY;
-                if (plan.newScores && row < live)
-                    storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[0], x[1], x[2], x[3]});
-                probabilities(t, x);
-                addValues(t, x);
-                for (int r = 0; r < 4; ++r) {
-                    unsigned long long holders = __ballot(odd >> r & 1);
-                    while (holders != 0) {
-                        const int group = (__ffsll(holders) - 1) >> 4;
-                        holders &= ~(0xFFFFull << (16 * group));
-                        const float weight = __shfl(x[r], group * 16 + i16, 64);
-                        const bool sees = __shfl(int(seen >> r & 1), group * 16 + i16, 64) != 0;
-                        const float* src = vn + size_t(j0 + 4 * group + r) * kvDim;
+            for (int r = 0; r < 4; ++r) x[t][r] = seen[t] >> r & 1 ? dots[r] : -INFINITY;
+            if (plan.newScores && row < live)
+                storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
+        }
+        probabilities(std::integral_constant<int, RT>{}, x);
 #pragma unroll
-                        for (int u = 0; u < VU; ++u)
+        for (int t = 0; t < RT; ++t) {
+            addValues(t, x[t]);
+            for (int r = 0; r < 4; ++r) {
+                unsigned long long holders = __ballot(odd >> r & 1);
+                while (holders != 0) {
+                    const int group = (__ffsll(holders) - 1) >> 4;
+                    holders &= ~(0xFFFFull << (16 * group));
+                    const float weight = __shfl(x[t][r], group * 16 + i16, 64);
+                    const bool sees = __shfl(int(seen[t] >> r & 1), group * 16 + i16, 64) != 0;
+                    const float* src = vn + size_t(j0 + 4 * group + r) * kvDim;
 #pragma unroll
-                            for (int w = 0; w < VW; ++w)
+                    for (int u = 0; u < VU; ++u)
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    const int d = u * 16 * VW + (4 * g + e) * VW + w;
-                                    const float value = d < hd ? src[d] : 0.0f;
-                                    if (sees && !(fabsf(value) < INFINITY)) o[t][u][w][e] += weight * value;
-                                }
-                    }
+                        for (int w = 0; w < VW; ++w)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int d = u * 16 * VW + (4 * g + e) * VW + w;
+                                const float value = d < hd ? src[d] : 0.0f;
+                                if (sees && !(fabsf(value) < INFINITY)) o[t][u][w][e] += weight * value;
+                            }
                 }
             }
         }
@@ -397,13 +415,13 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         const int node = row / share, h = kh * share + row % share;
         const float inv = only ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
         float* dst = only ? p.out + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd
-                          : plan.partOut + ((size_t(item) * p.kvHeads + kh) * rows + row) * hd;
+                          : plan.partOut + ((size_t(item) * p.kvHeads + kh) * rows + row) * plan.partPitch;
         for (int d = part * 4; d < hd; d += 64) {
             float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) acc = acc + *reinterpret_cast<const float4v*>(smem + (w * RT * 16 + r) * PITCH + d) * f[w];
             acc = acc * inv;
-            if (MODE != 0) {
+            if (MODE != 0 || !only) {
                 storef4(dst + d, acc);
             } else {
                 for (int j = 0; j < 4; ++j)
@@ -417,45 +435,55 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     }
 }
 
-// The chunks of a row put together: a wavefront per (sequence, key head, row), lanes over the head's columns.
+// The chunks of a row put together.  LPR lanes hold a row's columns, four each, so that a wavefront reads 64 / LPR chunks at
+// once; WPR wavefronts share a row's chunks (one where the sequences have few, four where they have many).
+template <int LPR, int WPR>
 __global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan plan) {
-    const int lane = threadIdx.x & 63, share = p.heads / p.kvHeads, rows = p.nodes * share;
-    const size_t flat = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    constexpr int CPW = 64 / LPR, STEP = CPW * WPR;
+    __shared__ float4v sAcc[4][LPR];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = p.heads / p.kvHeads, rows = p.nodes * share;
+    const size_t flat = WPR == 4 ? blockIdx.x : size_t(blockIdx.x) * 4 + wave;
     if (flat >= size_t(p.batch) * p.kvHeads * rows) return;
     const int row = int(flat % rows), kh = int(flat / rows % p.kvHeads), b = int(flat / rows / p.kvHeads);
-    if (row >= nodesInUse(p, b) * share) return;
     const int2 span = plan.span[b];
-    if (span.y == 1) return;   // written by its only chunk
+    if (row >= nodesInUse(p, b) * share || span.y == 1) return;   // no such row, or written by its only chunk
     const size_t step = size_t(p.kvHeads) * rows, at = size_t(span.x) * step + size_t(kh) * rows + row;
+    const int sub = lane % LPR, first = (WPR == 4 ? wave * CPW : 0) + lane / LPR;
     float most = kNoRef, mx = -INFINITY, sum = 0.0f;
+    for (int c = lane; c < span.y; c += 64) most = fmaxf(most, plan.partStat[at + c * step].x);
+    most = waveMax(most);
     for (int c = lane; c < span.y; c += 64) {
         const float4v st = plan.partStat[at + c * step];
-        const float to = fmaxf(most, st.x);
-        sum = sum * __builtin_amdgcn_exp2f(most - to) + st.y * __builtin_amdgcn_exp2f(st.x - to);
-        most = to;
+        sum += st.y * __builtin_amdgcn_exp2f(st.x - most);
         mx = fmaxf(mx, st.z);
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const float other = __shfl_xor(most, off, 64), otherSum = __shfl_xor(sum, off, 64), to = fmaxf(most, other);
-        sum = sum * __builtin_amdgcn_exp2f(most - to) + otherSum * __builtin_amdgcn_exp2f(other - to);
-        most = to;
-        mx = fmaxf(mx, __shfl_xor(mx, off, 64));
-    }
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    sum = waveSum(sum);
+    mx = waveMax(mx);
+    float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool on = sub * 4 < p.hd;
 #pragma unroll 4
-    for (int c = 0; c < span.y; ++c) {
+    for (int c = first; c < span.y; c += STEP) {
         const float f = __builtin_amdgcn_exp2f(plan.partStat[at + c * step].x - most);
-        const float* src = plan.partOut + (at + c * step) * p.hd;
+        const float4v x = on ? loadf4(plan.partOut + (at + c * step) * plan.partPitch + sub * 4) : float4v{0.0f, 0.0f, 0.0f, 0.0f};
+        acc = acc + x * f;
+    }
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (lane + 64 * j < p.hd) acc[j] += f * src[lane + 64 * j];
+    for (int off = LPR; off < 64; off <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], off, 64);
+    if constexpr (WPR == 4) {
+        if (lane < LPR) sAcc[wave][lane] = acc;
+        __syncthreads();
+        if (wave != 0) return;
+        acc = (sAcc[0][sub] + sAcc[1][sub]) + (sAcc[2][sub] + sAcc[3][sub]);
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float* dst = p.out + (size_t(b) * p.nodes + row / share) * p.heads * p.hd + size_t(kh * share + row % share) * p.hd;
+    float* dst = p.out + (size_t(b) * p.nodes + row / share) * p.heads * p.hd + size_t(kh * share + row % share) * p.hd + sub * 4;
+    if (lane < LPR) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (lane + 64 * j < p.hd) dst[lane + 64 * j] = acc[j] * inv;
+        for (int j = 0; j < 4; ++j)
+            if (sub * 4 + j < p.hd) dst[j] = acc[j] * inv;
+    }
     if (lane == 0) finishStats(p, plan, b, kh, row, most, sum, mx);
 }
 
@@ -841,25 +869,34 @@ int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
     return BF_OK;
 }
 
-template <int HDP, int RT, int MODE>
+template <int HDP, int RT, int MODE, bool SCORES>
 int launchTilesOf(const TreeParams& p, const TilePlan& plan, unsigned grid, hipStream_t s) {
     constexpr size_t smem = size_t(4) * RT * 16 * (HDP + 4) * sizeof(float);
-    const int st = allowDynamicSharedMemory(reinterpret_cast<const void*>(treeTilesKernel<HDP, RT, MODE>), smem);
+    const int st = allowDynamicSharedMemory(reinterpret_cast<const void*>(treeTilesKernel<HDP, RT, MODE, SCORES>), smem);
     if (st != BF_OK) return st;
-    treeTilesKernel<HDP, RT, MODE><<<grid, 256, smem, s>>>(p, plan);
+    treeTilesKernel<HDP, RT, MODE, SCORES><<<grid, 256, smem, s>>>(p, plan);
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
 template <int HDP, int RT>
 int launchTilesMode(const TreeParams& p, const TilePlan& plan, int mode, unsigned grid, hipStream_t s) {
-    if (mode == 2) return launchTilesOf<HDP, RT, 2>(p, plan, grid, s);
-    if (mode == 1) return launchTilesOf<HDP, RT, 1>(p, plan, grid, s);
-    return launchTilesOf<HDP, RT, 0>(p, plan, grid, s);
+    if constexpr (RT == 1) {   // dot products are kept for up to 16 rows only
+        if (plan.scores) {
+            if (mode == 2) return launchTilesOf<HDP, RT, 2, true>(p, plan, grid, s);
+            if (mode == 1) return launchTilesOf<HDP, RT, 1, true>(p, plan, grid, s);
+            return launchTilesOf<HDP, RT, 0, true>(p, plan, grid, s);
+        }
+    }
+    if (mode == 2) return launchTilesOf<HDP, RT, 2, false>(p, plan, grid, s);
+    if (mode == 1) return launchTilesOf<HDP, RT, 1, false>(p, plan, grid, s);
+    return launchTilesOf<HDP, RT, 0, false>(p, plan, grid, s);
 }
 template <int HDP>
 int launchTilesRows(const TreeParams& p, const TilePlan& plan, int rt, int mode, unsigned grid, hipStream_t s) {
-    if constexpr (HDP <= 128) {
+    if constexpr (HDP <= 64) {
         if (rt == 4) return launchTilesMode<HDP, 4>(p, plan, mode, grid, s);
+    }
+    if constexpr (HDP <= 128) {
         if (rt == 2) return launchTilesMode<HDP, 2>(p, plan, mode, grid, s);
     }
     return launchTilesMode<HDP, 1>(p, plan, mode, grid, s);
@@ -872,6 +909,21 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
         case 192: return launchTilesRows<192>(p, plan, rt, mode, grid, s);
         default: return launchTilesRows<256>(p, plan, rt, mode, grid, s);
     }
+}
+
+template <int LPR>
+int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, hipStream_t s) {
+    // chunks a sequence has on average: four wavefronts a row once one would go round more than four times
+    if (size_t(plan.items) > size_t(p.batch) * 4 * (64 / LPR)) treeJoinKernel<LPR, 4><<<unsigned(rows), 256, 0, s>>>(p, plan);
+    else treeJoinKernel<LPR, 1><<<unsigned((rows + 3) / 4), 256, 0, s>>>(p, plan);
+    BF_LAUNCH_CHECK();
+    return BF_OK;
+}
+int launchJoin(const TreeParams& p, const TilePlan& plan, size_t rows, hipStream_t s) {
+    if (p.hd <= 32) return launchJoinOf<8>(p, plan, rows, s);
+    if (p.hd <= 64) return launchJoinOf<16>(p, plan, rows, s);
+    if (p.hd <= 128) return launchJoinOf<32>(p, plan, rows, s);
+    return launchJoinOf<64>(p, plan, rows, s);
 }
 
 int checkHeads(const char* fn, size_t heads, size_t kvHeads, size_t groups, size_t headDim) {
@@ -901,19 +953,20 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const bool recompute = weights && capacity != 0 && !keepScores;
     // Row tiles a wavefront holds: what the rows fill, up to the registers there are
     const int hdp = paddedHeadDim(headDim);
-    const int most = hdp <= 128 ? 4 : 1;
-    const int rt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
+    const int most = hdp <= 64 ? 4 : hdp <= 128 ? 2 : 1;
+    const int rt = std::min(getenv("RT") ? std::min(most,atoi(getenv("RT"))) : most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
     TilePlan plan{};
     plan.rowGroups = int((rows + 16 * rt - 1) / (16 * rt));
-    plan.minChunk = 128;
-    plan.target = int(std::max<size_t>(1, size_t(computeUnits()) * 4 / (kvHeads * size_t(plan.rowGroups))));
+    plan.minChunk = getenv("MC") ? atoi(getenv("MC")) : 128;
+    plan.target = int(std::max<size_t>(1, size_t(computeUnits()) * (getenv("WF") ? atoi(getenv("WF")) : 4) / (kvHeads * size_t(plan.rowGroups))));
     const size_t chunksAtMost = batch * std::max<size_t>(1, (capacity + plan.minChunk - 1) / plan.minChunk);
     plan.items = int(std::min(chunksAtMost, size_t(plan.target) + batch));
     plan.c = float(std::fabs(double(p.scale)) * 1.4426950408889634074);
     plan.scorePitch = int((capacity + 15) / 16 * 16);
+    plan.partPitch = int((headDim + 3) / 4 * 4);
     const bool join = size_t(plan.items) > batch;
     const size_t slots = size_t(plan.items) * kvHeads * rows, rowsAll = batch * kvHeads * rows;
-    const size_t need[] = {join ? slots * sizeof(float4v) : 0, join ? slots * headDim * sizeof(float) : 0, batch * sizeof(int2),
+    const size_t need[] = {join ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
                            keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, weights ? rowsAll * 64 * sizeof(float) : 0,
                            weights ? rowsAll * sizeof(float2) : 0, recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
     size_t bytes = 0, offset[7];
@@ -939,8 +992,8 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     st = launchTiles(p, plan, hdp, rt, mode, grid, s);
     if (st != BF_OK) return st;
     if (join) {
-        treeJoinKernel<<<unsigned((rowsAll + 3) / 4), 256, 0, s>>>(p, plan);
-        BF_LAUNCH_CHECK();
+        st = launchJoin(p, plan, rowsAll, s);
+        if (st != BF_OK) return st;
     }
     if (weights && capacity != 0) {
         // the new rows' weights, and the cached rows' where their dot products were kept
