@@ -69,11 +69,12 @@ struct TilePlan {
 
 // Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for
 // each.  Returns this item's sequence (-1: there is none) and its chunk.
-struct Chunk { int b, first, count, start, end; };
+struct Chunk { int b, first, count, start, end, queries; };
 __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& plan, int item) {
     const int lane = threadIdx.x & 63;
-    long long total = 0;   // in units of 64 rows
-    for (int b0 = 0; b0 < p.batch; b0 += 64) total += b0 + lane < p.batch ? (rowsInUse(p, b0 + lane) + 63) / 64 : 0;
+    const int length0 = lane < p.batch ? rowsInUse(p, lane) : 0, count0 = lane < p.batch ? nodesInUse(p, lane) : 0;
+    long long total = (length0 + 63) / 64;   // in units of 64 rows
+    for (int b0 = 64; b0 < p.batch; b0 += 64) total += b0 + lane < p.batch ? (rowsInUse(p, b0 + lane) + 63) / 64 : 0;
     if (p.batch > 1) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
@@ -82,26 +83,33 @@ __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& 
     }
     const int even = int(min((total + plan.target - 1) / plan.target, (long long)(1 << 24)));
     const int size = max(plan.minChunk, even * 64);
-    Chunk c{-1, 0, 0, 0, 0};
+    Chunk c{-1, 0, 0, 0, 0, 0};
     int before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        const int length = b0 + lane < p.batch ? rowsInUse(p, b0 + lane) : 0;
-        const int mine = b0 + lane < p.batch ? max(1, (length + size - 1) / size) : 0;
+        const bool on = b0 + lane < p.batch;
+        const int length = b0 == 0 ? length0 : on ? rowsInUse(p, b0 + lane) : 0;
+        const int count = b0 == 0 ? count0 : on ? nodesInUse(p, b0 + lane) : 0;
+        const int mine = on ? max(1, (length + size - 1) / size) : 0;
         int upTo = mine;
+        if (p.batch > 1) {
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int o = __shfl_up(upTo, off, 64);
-            if (lane >= off) upTo += o;
+            for (int off = 1; off < 64; off <<= 1) {
+                const int o = __shfl_up(upTo, off, 64);
+                if (lane >= off) upTo += o;
+            }
         }
-        const unsigned long long past = __ballot(before + upTo > item);
+        const unsigned long long past = __ballot(on && before + upTo > item);
         if (past != 0) {
             const int at = __ffsll(past) - 1;
             c.b = __builtin_amdgcn_readfirstlane(b0 + at);
             c.count = __builtin_amdgcn_readlane(mine, at);
             c.first = before + __builtin_amdgcn_readlane(upTo, at) - c.count;
+            c.queries = __builtin_amdgcn_readlane(count, at);
             const int len = __builtin_amdgcn_readlane(length, at);
-            c.start = (item - c.first) * size;
-            c.end = min(c.start + size, len);
+            // a sequence's chunks are of one size, a multiple of 64 rows
+            const int each = ((len + c.count - 1) / c.count + 63) / 64 * 64;
+            c.start = min((item - c.first) * each, len);
+            c.end = min(c.start + each, len);
             return c;
         }
         before += __builtin_amdgcn_readlane(upTo, 63);
@@ -150,6 +158,9 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     constexpr int VU = HDP / (16 * VW);             // such loads
     extern __shared__ float smem[];
     __shared__ float4v sStat[4][RT * 16];
+    __shared__ unsigned sOdd[4];   // new rows of each 16 that hold a value which is not finite
+    if (threadIdx.x < 4) sOdd[threadIdx.x] = 0;
+    __syncthreads();
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
     // the row groups of one chunk next to each other on one XCD (workgroups go to the 8 XCDs in turn), where they share its reads
     const unsigned perXcd = blockIdx.x / 8, flat = perXcd / plan.rowGroups * 8 + blockIdx.x % 8;
@@ -159,7 +170,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     const Chunk ch = findChunk(p, plan, item);
     if (ch.b < 0) return;
     const int b = ch.b, share = p.heads / p.kvHeads, rows = p.nodes * share, hd = p.hd;
-    const int count = nodesInUse(p, b), live = count * share;     // rows past `live` belong to no node
+    const int count = ch.queries, live = count * share;     // rows past `live` belong to no node
     if (item == ch.first && kh == 0 && rowGroup == 0 && threadIdx.x == 0) plan.span[b] = make_int2(ch.first, ch.count);
     const int row0 = rowGroup * RT * 16;
     if (row0 >= live) return;
@@ -167,6 +178,11 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     const size_t kvDim = size_t(p.kvHeads) * hd;
     const float* kb = p.k + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
     const float* vb = p.v + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
+
+    // With the sequence's last chunk go its new rows, 16 to a wavefront, starting with the one that has the fewest cached ones
+    const int newTile = (wave - (ch.end - ch.start + 15) / 16) & 3;
+    const bool hasNew = item == ch.first + ch.count - 1 && newTile * 16 < count;
+    unsigned seen[RT];   // bits 0..3: new rows 16 newTile + 4 g .. that this lane's row of tile t sees
 
     float q[RT][KS][4];
     const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
@@ -176,6 +192,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         const bool on = row < live;
         const int node = on ? row / share : 0, h = kh * share + (on ? row % share : 0);
         const float* src = p.q + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd;
+        seen[t] = hasNew && on ? unsigned(newRowsSeen(p, b, node, count) >> (newTile * 16 + 4 * g)) & 15u : 0u;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             loadColumns<MODE, 4>(q[t][s], src, 16 * s + 4 * g, hd);
@@ -315,61 +332,38 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         if (tiles == 2) walk(std::integral_constant<int, 2>{});
         if (tiles == 3) walk(std::integral_constant<int, 3>{});
     }
-    // new rows: with the sequence's last chunk, the wavefronts again taking 16 in turn
-    if (item == ch.first + ch.count - 1 && wave * 16 < count) {
-        const int j0 = wave * 16;
-        const float* kn = p.kNew + size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
-        const float* vn = p.vNew + size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
-        loadK(kn, j0, count - 1);
-        loadV(vn, j0, count - 1);
-        // values that are not finite must reach the rows that see them and no others: they are taken out of the products
-        unsigned odd = 0;   // bit r: this lane holds one of key 4 g + r
+    if (hasNew) {
+        const int j0 = newTile * 16;
+        const size_t at = size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
+        loadK(p.kNew + at, j0, count - 1);
+        loadV(p.vNew + at, j0, count - 1);
+        // A value that is not finite must not meet the weight zero of a row that does not see it: taken out here, added to
+        // the rows that do when the results are written.
+        unsigned notFinite = 0;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
-                    if (j0 + 4 * g + r >= count) v[u][r][w] = 0.0f;
-                    if (!(fabsf(v[u][r][w]) < INFINITY)) { odd |= 1u << r; v[u][r][w] = 0.0f; }
+                    const bool in = j0 + 4 * g + r < count, finite = fabsf(v[u][r][w]) < INFINITY;
+                    if (in && !finite) notFinite |= 1u << (4 * g + r);
+                    v[u][r][w] = in && finite ? v[u][r][w] : 0.0f;
                 }
+        if (notFinite) atomicOr(&sOdd[newTile], notFinite);
         float x[RT][4];
-        unsigned long long seen[RT];
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int row = row0 + t * 16 + i16;
-            seen[t] = row < live ? newRowsSeen(p, b, row / share, count) >> j0 >> (4 * g) : 0ull;
             const float4v dots = dotProducts(t);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[t][r] = seen[t] >> r & 1 ? dots[r] : -INFINITY;
+            const int row = row0 + t * 16 + i16;
             if (plan.newScores && row < live)
                 storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
         }
         probabilities(std::integral_constant<int, RT>{}, x);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            addValues(t, x[t]);
-            for (int r = 0; r < 4; ++r) {
-                unsigned long long holders = __ballot(odd >> r & 1);
-                while (holders != 0) {
-                    const int group = (__ffsll(holders) - 1) >> 4;
-                    holders &= ~(0xFFFFull << (16 * group));
-                    const float weight = __shfl(x[t][r], group * 16 + i16, 64);
-                    const bool sees = __shfl(int(seen[t] >> r & 1), group * 16 + i16, 64) != 0;
-                    const float* src = vn + size_t(j0 + 4 * group + r) * kvDim;
-#pragma unroll
-                    for (int u = 0; u < VU; ++u)
-#pragma unroll
-                        for (int w = 0; w < VW; ++w)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int d = u * 16 * VW + (4 * g + e) * VW + w;
-                                const float value = d < hd ? src[d] : 0.0f;
-                                if (sees && !(fabsf(value) < INFINITY)) o[t][u][w][e] += weight * value;
-                            }
-                }
-            }
-        }
+        for (int t = 0; t < RT; ++t) addValues(t, x[t]);
     }
 
     // the four wavefronts' states joined through LDS, [wave][row][HDP + 4]
@@ -387,13 +381,16 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
 #pragma unroll
             for (int u = 0; u < VU; ++u)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w) mine[u * 16 * VW + (4 * g + e) * VW + w] = o[t][u][w][e];
+                for (int e = 0; e < 4; ++e) {
+                    float* to = mine + u * 16 * VW + (4 * g + e) * VW;
+                    if constexpr (VW == 4) storef4(to, float4v{o[t][u][0][e], o[t][u][1][e], o[t][u][2][e], o[t][u][3][e]});
+                    else *reinterpret_cast<float2v*>(to) = float2v{o[t][u][0][e], o[t][u][1][e]};
+                }
         }
     }
     __syncthreads();
     const bool only = ch.count == 1;
+    const unsigned long long odd = (unsigned long long)(sOdd[0] | sOdd[1] << 16) | (unsigned long long)(sOdd[2] | sOdd[3] << 16) << 32;
     const int liveHere = min(live - row0, tiles * 16);
     // sixteen threads a row, four columns at a time
     for (int e = threadIdx.x; e < liveHere * 16; e += 256) {
@@ -421,6 +418,13 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
 #pragma unroll
             for (int w = 0; w < 4; ++w) acc = acc + *reinterpret_cast<const float4v*>(smem + (w * RT * 16 + r) * PITCH + d) * f[w];
             acc = acc * inv;
+            if (odd != 0) {
+                for (unsigned long long left = odd & newRowsSeen(p, b, node, count); left != 0; left &= left - 1) {
+                    const float* src = p.vNew + (size_t(b) * p.nodes + __ffsll(left) - 1) * kvDim + size_t(kh) * hd + d;
+                    for (int j = 0; j < 4; ++j)
+                        if (d + j < hd && !(fabsf(src[j]) < INFINITY)) acc[j] += src[j];
+                }
+            }
             if (MODE != 0 || !only) {
                 storef4(dst + d, acc);
             } else {
