@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <initializer_list>
 
 namespace bf {
 namespace {
@@ -36,10 +37,13 @@ __device__ __forceinline__ unsigned weightKey(float w) {
 // rows.  Two more passes write the kept rows in order: the wavefronts own consecutive stretches, count, and then emit at
 // the offsets that the counts before them give.  Last the kept rows' weights move up, a tile at a time, all of a
 // tile's reads before its writes: row i comes from a row at or after i, so a call in place overwrites nothing unread.
+// With NK > 0 the capacity is at most 1024 NK and a thread keeps its NK keys in registers, so the weights are read once
+// (8 sequences of 16384 rows, 16 groups: 33 us reading them in every pass); NK = 0 reads them again.
+template <int NK>
 __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
     constexpr int BINS = 2048, WAVES = 16;
     __shared__ unsigned hist[BINS];
-    __shared__ unsigned total[1024 / 64];
+    __shared__ unsigned total[WAVES];
     __shared__ unsigned sDigit, sAbove;
     __shared__ int sGreater[WAVES], sEqual[WAVES];
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
@@ -53,6 +57,26 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
         for (int i = t; i < left; i += 1024) kept[i] = i;
     } else {
         const int n = length - p.recent, places = p.budget - p.recent;   // n > places >= 0
+        // wavefront's stretch; element e of a lane is row from + 64 e + lane
+        const int stretch = NK > 0 ? NK * 64 : ((n + WAVES - 1) / WAVES + 63) / 64 * 64;
+        const int from = min(wave * stretch, n), to = min(from + stretch, n);
+        unsigned key[NK > 0 ? NK : 1];
+        if constexpr (NK > 0) {
+            float x[NK];
+#pragma unroll
+            for (int e = 0; e < NK; ++e) x[e] = w[min(from + 64 * e + lane, n - 1)];
+#pragma unroll
+            for (int e = 0; e < NK; ++e) key[e] = weightKey(x[e]);
+        }
+        auto each = [&](auto f) {   // f(row, key, the row exists): called by whole wavefronts
+            if constexpr (NK > 0) {
+#pragma unroll
+                for (int e = 0; e < NK; ++e)
+                    if (from + 64 * e < to) f(from + 64 * e + lane, key[e], from + 64 * e + lane < to);
+            } else {
+                for (int i0 = from; i0 < to; i0 += 64) f(i0 + lane, weightKey(w[min(i0 + lane, n - 1)]), i0 + lane < to);
+            }
+        };
         unsigned prefix = 0;     // the digits found so far
         int need = places;       // places left for keys that share them
         int shift = 32;
@@ -62,12 +86,11 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
                 shift -= bits;
                 for (int i = t; i < BINS; i += 1024) hist[i] = 0;
                 __syncthreads();
-                for (int i = t; i < n; i += 1024) {
-                    const unsigned key = weightKey(w[i]);
-                    if (pass == 0 || key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
-                }
+                each([&](int, unsigned x, bool in) {
+                    if (in && (pass == 0 || x >> (shift + bits) == prefix)) atomicAdd(&hist[x >> shift & ((1u << bits) - 1)], 1u);
+                });
                 __syncthreads();
-                // bins from the top: thread t owns the pair of bins below 2 t others, a suffix sum finds the one with place `need`
+                // thread t owns a pair of bins, 2 t bins from the top: the bin that holds place `need`
                 const int hi = BINS - 1 - 2 * t, lo = hi - 1;
                 const unsigned a = hist[hi], c = hist[lo];
                 unsigned sum = a + c;
@@ -79,7 +102,8 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
                 if (lane == 63) total[wave] = sum;
                 __syncthreads();
                 unsigned before = sum - a - c;
-                for (int x = 0; x < wave; ++x) before += total[x];
+#pragma unroll
+                for (int x = 0; x < WAVES; ++x) before += x < wave ? total[x] : 0u;
                 if (before < unsigned(need) && before + a >= unsigned(need)) { sDigit = hi; sAbove = before; }
                 else if (before + a < unsigned(need) && before + a + c >= unsigned(need)) { sDigit = lo; sAbove = before + a; }
                 __syncthreads();
@@ -89,46 +113,46 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
             }
         }
         // keys above `prefix` stay, and the first `need` of those equal to it
-        const int stretch = ((n + WAVES - 1) / WAVES + 63) / 64 * 64;
-        const int from = min(wave * stretch, n), to = min(from + stretch, n);
         int greater = 0, equal = 0;
         if (places > 0) {
-            for (int i0 = from; i0 < to; i0 += 64) {
-                const int i = i0 + lane;
-                const unsigned key = i < to ? weightKey(w[i]) : 0u;
-                greater += __popcll(__ballot(i < to && key > prefix));
-                equal += __popcll(__ballot(i < to && key == prefix));
-            }
+            each([&](int, unsigned x, bool in) {
+                greater += __popcll(__ballot(in && x > prefix));
+                equal += __popcll(__ballot(in && x == prefix));
+            });
         }
         if (lane == 0) { sGreater[wave] = greater; sEqual[wave] = equal; }
         __syncthreads();
         int at = 0, equalBefore = 0;
-        for (int x = 0; x < wave; ++x) {
-            at += sGreater[x] + min(max(need - equalBefore, 0), sEqual[x]);
-            equalBefore += sEqual[x];
+#pragma unroll
+        for (int x = 0; x < WAVES; ++x) {
+            if (x < wave) {
+                at += sGreater[x] + min(max(need - equalBefore, 0), sEqual[x]);
+                equalBefore += sEqual[x];
+            }
         }
         if (places > 0) {
             const unsigned long long below = (1ull << lane) - 1;
-            for (int i0 = from; i0 < to; i0 += 64) {
-                const int i = i0 + lane;
-                const unsigned key = i < to ? weightKey(w[i]) : 0u;
-                const unsigned long long eq = __ballot(i < to && key == prefix);
-                const bool stays = i < to && (key > prefix || (key == prefix && equalBefore + __popcll(eq & below) < need));
+            each([&](int i, unsigned x, bool in) {
+                const unsigned long long eq = __ballot(in && x == prefix);
+                const bool stays = in && (x > prefix || (x == prefix && equalBefore + __popcll(eq & below) < need));
                 const unsigned long long st = __ballot(stays);
                 if (stays) kept[at + __popcll(st & below)] = i;
                 at += __popcll(st);
                 equalBefore += __popcll(eq);
-            }
+            });
         }
         for (int i = t; i < p.recent; i += 1024) kept[places + i] = n + i;
     }
     __syncthreads();   // kept[] is read back below by other threads of this workgroup
     float* wOut = p.weightsOut + (size_t(b) * p.groups + g) * p.outCapacity;
-    for (int i0 = 0; i0 < left; i0 += 1024) {
-        const int i = i0 + t;
-        const float x = i < left ? w[kept[i]] : 0.0f;
+    for (int i0 = 0; i0 < left; i0 += 4096) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) x[u] = i0 + 1024 * u + t < left ? w[kept[i0 + 1024 * u + t]] : 0.0f;
         __syncthreads();
-        if (i < left) wOut[i] = x;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (i0 + 1024 * u + t < left) wOut[i0 + 1024 * u + t] = x[u];
     }
 }
 
@@ -183,41 +207,69 @@ __global__ void __launch_bounds__(256) evictMoveKernel(EvictParams p, int slices
 }
 
 // ---- verification of a drafted tree ------------------------------------------------------------
-// Lowest index of a row's maximum; a NaN is never chosen unless it is element 0, which is then never beaten (the loop
-// "best = 0; if (row[c] > row[best]) best = c").
-__device__ __forceinline__ float choiceKey(float v, int i) { return v != v ? (i == 0 ? INFINITY : -INFINITY) : v; }
-
-__global__ void __launch_bounds__(1024) treeChoiceKernel(const float* __restrict__ logits, const int* __restrict__ counts, int* __restrict__ choice,
-                                                         int nodes, int vocab) {
-    __shared__ float vals[16];
-    __shared__ int idxs[16];
-    const int b = blockIdx.x / nodes, i = blockIdx.x % nodes;
+// Lowest index of each row's maximum, by the loop "best = 0; if (row[c] > row[best]) best = c": a NaN is never chosen unless
+// it is element 0, which is then never beaten.  The logits are read once, 16 bytes a thread and four loads in flight, and
+// compared in groups of four: of the best group only the value and the place are kept until the end.  `pieces` workgroups
+// share a row where there are few rows (26 rows of 50257: 13.7 us with one each).
+struct Best { float value; int at; };   // at: INT_MAX, nothing above -infinity seen
+__device__ __forceinline__ void take(Best& mine, float value, int at) {
+    if (value > mine.value || (value == mine.value && at < mine.at)) { mine.value = value; mine.at = at; }
+}
+__global__ void __launch_bounds__(256) treeChoiceKernel(const float* __restrict__ logits, const int* __restrict__ counts, Best* __restrict__ best,
+                                                        int nodes, int vocab, int pieces) {
+    __shared__ Best sBest[4];
+    const int row = blockIdx.x / pieces, piece = blockIdx.x % pieces, b = row / nodes, i = row % nodes;
     if (counts && i >= counts[b]) return;
-    const float* row = logits + size_t(blockIdx.x) * vocab;
-    float best = -INFINITY;
-    int at = INT_MAX;
-    for (int c = threadIdx.x; c < vocab; c += 1024) {
-        const float v = choiceKey(row[c], c);
-        if (v > best || at == INT_MAX) { best = v; at = c; }
+    const float* x = logits + size_t(row) * vocab;
+    // groups of four from the 16-byte boundary at or below the row's first element; the row's ends are taken one by one
+    const int shift = int((reinterpret_cast<uintptr_t>(x) >> 2) & 3), groups = (vocab + shift + 3) / 4;
+    const int per = (groups + pieces - 1) / pieces, from = piece * per, to = min(from + per, groups);
+    auto whole = [&](int group) { return group * 4 >= shift && group * 4 + 4 <= vocab + shift; };
+    auto load = [&](int group) {
+        if (whole(group)) return loadf4(x + (group * 4 - shift));
+        float4v v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int c = group * 4 - shift + j;
+            v[j] = c >= 0 && c < vocab ? x[c] : -INFINITY;
+        }
+        return v;
+    };
+    Best mine{-INFINITY, INT_MAX};
+    for (int g0 = from + int(threadIdx.x); g0 < to; g0 += 1024) {
+        float4v v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = g0 + 256 * u < to ? load(g0 + 256 * u) : float4v{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float most = fmaxf(fmaxf(v[u].x, v[u].y), fmaxf(v[u].z, v[u].w));   // fmaxf passes over NaN
+            if (most > mine.value) { mine.value = most; mine.at = g0 + 256 * u; }
+        }
     }
-    auto take = [&](float v, int j) { if (j != INT_MAX && (at == INT_MAX || v > best || (v == best && j < at))) { best = v; at = j; } };
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) {
-        const float v = __shfl_xor(best, off, 64);
-        const int j = __shfl_xor(at, off, 64);
-        take(v, j);
+        const float value = __shfl_xor(mine.value, off, 64);
+        const int at = __shfl_xor(mine.at, off, 64);
+        take(mine, value, at);
     }
-    if ((threadIdx.x & 63) == 0) { vals[threadIdx.x >> 6] = best; idxs[threadIdx.x >> 6] = at; }
+    if ((threadIdx.x & 63) == 0) sBest[threadIdx.x >> 6] = mine;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int x = 1; x < 16; ++x) take(vals[x], idxs[x]);
-        choice[blockIdx.x] = at;
+        for (int w = 1; w < 4; ++w) take(mine, sBest[w].value, sBest[w].at);
+        if (mine.at != INT_MAX) {
+            const float4v v = load(mine.at);
+            int j = 0;
+            while (j < 3 && !(v[j] == mine.value)) ++j;
+            mine.at = mine.at * 4 - shift + j;
+        }
+        if (piece == 0 && x[0] != x[0]) mine = Best{INFINITY, 0};
+        best[blockIdx.x] = mine;
     }
 }
 
 // One wavefront per sequence, a lane per node: from the root, the lowest-numbered child that carries the token chosen at
 // the node, until there is none.  Children come after their parent, so the walk ends.
-__global__ void __launch_bounds__(64) treeWalkKernel(const int* __restrict__ choice, const float* __restrict__ tokens, const int* __restrict__ parents,
+__global__ void __launch_bounds__(64) treeWalkKernel(const Best* __restrict__ best, int pieces, const float* __restrict__ tokens, const int* __restrict__ parents,
                                                      const int* __restrict__ counts, int* __restrict__ path, int* __restrict__ pathCounts,
                                                      float* __restrict__ next, int nodes) {
     const int lane = threadIdx.x, b = blockIdx.x;
@@ -226,7 +278,12 @@ __global__ void __launch_bounds__(64) treeWalkKernel(const int* __restrict__ cho
     const bool live = lane < count;
     const int parent = live ? parents[at] : -1;
     const long token = live ? lroundf(tokens[at]) : -1;
-    const int mine = live ? choice[at] : -1;
+    Best chosenHere{-INFINITY, INT_MAX};
+    for (int x = 0; live && x < pieces; ++x) {
+        const Best piece = best[at * pieces + x];
+        take(chosenHere, piece.value, piece.at);
+    }
+    const int mine = chosenHere.at == INT_MAX ? 0 : chosenHere.at;   // nothing above -infinity: element 0 was never beaten
     int found = 0, cur = 0, step = -1;     // `step`: what this lane writes into path[lane]
     if (count > 0) {
         for (;;) {
@@ -329,7 +386,11 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
     if (own.status != BF_OK) return own.status;
     p.left = own.as<int>();
     p.kept = kept ? kept : p.left + batch;
-    evictSelectKernel<<<unsigned(batch * groups), 1024, 0, s>>>(p);
+    const unsigned pairs = unsigned(batch * groups);
+    if (capacity <= 4 * 1024) evictSelectKernel<4><<<pairs, 1024, 0, s>>>(p);
+    else if (capacity <= 16 * 1024) evictSelectKernel<16><<<pairs, 1024, 0, s>>>(p);
+    else if (capacity <= 64 * 1024) evictSelectKernel<64><<<pairs, 1024, 0, s>>>(p);
+    else evictSelectKernel<0><<<pairs, 1024, 0, s>>>(p);
     BF_LAUNCH_CHECK();
     const bool vec = p.slab % 4 == 0 && aligned16(kCache) && aligned16(vCache) && aligned16(kOut) && aligned16(vOut);
     const int slices = std::max(1, (p.slab / (vec ? 4 : 1) + 15) / 16);
@@ -351,11 +412,14 @@ int bf_hip_tree_accept(const float* logits, const float* tokens, const int* pare
     BF_REQUIRE(vocab <= (size_t(1) << 24), "a token id beyond 2^24 has no exact float");
     BF_REQUIRE(logits && tokens && parents && path && pathCounts && next, "NULL pointer");
     hipStream_t s = asStream(stream);
-    Scratch choice(batch * nodes * sizeof(int));
-    if (choice.status != BF_OK) return choice.status;
-    treeChoiceKernel<<<unsigned(batch * nodes), 1024, 0, s>>>(logits, counts, choice.as<int>(), int(nodes), int(vocab));
+    // two workgroups a compute unit, as long as each has 4096 logits
+    const size_t rows = batch * nodes, wanted = (2 * size_t(computeUnits()) + rows - 1) / rows;
+    const size_t pieces = std::max<size_t>(1, std::min<size_t>({wanted, vocab / 4096, 32}));
+    Scratch best(rows * pieces * sizeof(Best));
+    if (best.status != BF_OK) return best.status;
+    treeChoiceKernel<<<unsigned(rows * pieces), 256, 0, s>>>(logits, counts, best.as<Best>(), int(nodes), int(vocab), int(pieces));
     BF_LAUNCH_CHECK();
-    treeWalkKernel<<<unsigned(batch), 64, 0, s>>>(choice.as<int>(), tokens, parents, counts, path, pathCounts, next, int(nodes));
+    treeWalkKernel<<<unsigned(batch), 64, 0, s>>>(best.as<Best>(), int(pieces), tokens, parents, counts, path, pathCounts, next, int(nodes));
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
@@ -391,7 +455,9 @@ int bf_hip_kv_commit(float* const* kCaches, float* const* vCaches, const float* 
         }
         p.lengthsOut = !lengthsDone && lengthsOut != lengths ? lengthsOut : nullptr;
         lengthsDone = lengthsDone || p.lengthsOut != nullptr;
-        const unsigned pieces = unsigned(std::min<size_t>(16, (nodes * rowFloats / (vec ? 4 : 1) + 255) / 256));
+        // workgroups for four rows at once: a path is rarely longer, and a workgroup without a row still costs its launch
+        // (32 sequences, 12 layers: 15 us with a workgroup for every row there might be)
+        const unsigned pieces = unsigned(std::min<size_t>(16, (std::min<size_t>(nodes, 4) * rowFloats / (vec ? 4 : 1) + 255) / 256));
         const dim3 grid(std::max(1u, pieces), unsigned(2 * n), unsigned(batch));
         if (vec) kvCommitKernel<4><<<grid, 256, 0, s>>>(p);
         else kvCommitKernel<1><<<grid, 256, 0, s>>>(p);
