@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
 // among themselves when the result goes to other tensors (each tile is then on its own).  In place one workgroup walks
 // all the tiles: a tile's reads come before the barrier, its writes after it, and what later tiles read lies at or
 // after their own first row.
-template <int VEC>
+template <int VEC, bool NT>
 __global__ void __launch_bounds__(256) evictMoveKernel(EvictParams p, int slices, int splits) {
     constexpr int ROWS = 16, U = 8, TILE = ROWS * U;
     const int slice = blockIdx.x % slices, side = blockIdx.x / slices % 2, split = blockIdx.x / slices / 2;
@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(256) evictMoveKernel(EvictParams p, int slices
             if (live && i < left) {
                 const float* from = src + size_t(kept[i]) * rowFloats;
                 if constexpr (VEC == 4) {
-                    const float4v f = loadf4(from);
+                    const float4v f = ldf4<NT>(from);
                     x[u][0] = f.x; x[u][1] = f.y; x[u][2] = f.z; x[u][3] = f.w;
                 } else {
                     x[u][0] = *from;
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(256) evictMoveKernel(EvictParams p, int slices
             const int i = i0 + u * ROWS + r0;
             if (live && i < left) {
                 float* to = dst + size_t(i) * rowFloats;
-                if constexpr (VEC == 4) storef4(to, float4v{x[u][0], x[u][1], x[u][2], x[u][3]});
+                if constexpr (VEC == 4) stf4<NT>(to, float4v{x[u][0], x[u][1], x[u][2], x[u][3]});
                 else *to = x[u][0];
             }
         }
@@ -397,8 +397,11 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
     const size_t tiles = std::max<size_t>(1, (std::min(budget, capacity) + 127) / 128);
     const int splits = inPlace ? 1 : int(std::min<size_t>(tiles, 64));
     const dim3 grid(unsigned(slices) * 2 * unsigned(splits), unsigned(groups), unsigned(batch));
-    if (vec) evictMoveKernel<4><<<grid, 256, 0, s>>>(p, slices, splits);
-    else evictMoveKernel<1><<<grid, 256, 0, s>>>(p, slices, splits);
+    // rows that stream past the last-level cache carry the non-temporal hint (0.9 GB moved: 195 -> 185 us with the selection)
+    const size_t moved = batch * std::min(budget, capacity) * groups * size_t(p.slab) * 4 * sizeof(float);
+    if (vec && streamsPastCache(moved)) evictMoveKernel<4, true><<<grid, 256, 0, s>>>(p, slices, splits);
+    else if (vec) evictMoveKernel<4, false><<<grid, 256, 0, s>>>(p, slices, splits);
+    else evictMoveKernel<1, false><<<grid, 256, 0, s>>>(p, slices, splits);
     BF_LAUNCH_CHECK();
     return BF_OK;
 }

@@ -61,8 +61,7 @@ struct TilePlan {
     int2* span;          // [batch]: first item and number of items of a sequence
     float* scores;       // [batch][kvHeads][rows][scorePitch] dot products with the cached rows (NULL: not kept)
     float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
-    float2* stat2;       // [batch][kvHeads][rows]: ref and 1 / l of the whole row, for the account of the weights
-    int scorePitch, partPitch;
+    int scorePitch, partPitch, keyBlocks;
     float c;             // |scale| log2(e)
 };
 
@@ -142,7 +141,6 @@ __device__ __forceinline__ void finishStats(const TreeParams& p, const TilePlan&
     const bool empty = sum == 0.0f;
     if (p.m) p.m[stat] = empty ? -INFINITY : top * fabsf(p.scale);
     if (p.l) p.l[stat] = empty ? 0.0f : sum * __builtin_amdgcn_exp2f(-fmaf(top, plan.c, -ref));
-    if (plan.stat2) plan.stat2[(size_t(b) * p.kvHeads + kh) * p.nodes * share + row] = make_float2(ref, empty ? 0.0f : 1.0f / sum);
 }
 
 constexpr float kNoRef = -3.402823466e38f;   // a reference below every score: the first real one moves it
@@ -433,17 +431,84 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         }
         if (part == 0) {
             if (only) finishStats(p, plan, b, kh, row, most, sum, mx);
-            else plan.partStat[(size_t(item) * p.kvHeads + kh) * rows + row] = float4v{most, sum, mx, 0.0f};
+            if (plan.partStat) plan.partStat[(size_t(item) * p.kvHeads + kh) * rows + row] = float4v{most, sum, mx, 0.0f};
         }
     }
 }
 
+// A row's reference and sum over its chunks, by a wavefront; `at` + c * `step` is chunk c's entry
+__device__ __forceinline__ float2 joinedSum(const TilePlan& plan, size_t at, size_t step, int chunks, float& mx) {
+    const int lane = threadIdx.x & 63;
+    float most = kNoRef, sum = 0.0f;
+    for (int c = lane; c < chunks; c += 64) most = fmaxf(most, plan.partStat[at + c * step].x);
+    most = waveMax(most);
+    mx = -INFINITY;
+    for (int c = lane; c < chunks; c += 64) {
+        const float4v st = plan.partStat[at + c * step];
+        sum += st.y * __builtin_amdgcn_exp2f(st.x - most);
+        mx = fmaxf(mx, st.z);
+    }
+    mx = waveMax(mx);
+    return make_float2(most, waveSum(sum));
+}
+
+// The weights of a block of 1024 cached rows, four a thread, from the kept dot products of the group's rows; the block of
+// the first ones also makes the new rows'.  The statistics are put together here once more, 64 rows at a time, rather than
+// waited for in a launch of their own (a step over 1500 rows, 12 heads: 15 -> 12 us).
+__device__ __forceinline__ void weightsFromScores(const TreeParams& p, const TilePlan& plan, int index) {
+    __shared__ float2 sStat[64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int block = index % plan.keyBlocks, g = index / plan.keyBlocks % p.groups, b = index / plan.keyBlocks / p.groups;
+    const int share = p.heads / p.kvHeads, rows = p.nodes * share, length = rowsInUse(p, b), count = nodesInUse(p, b), live = count * share;
+    if (block != 0 && block * 1024 >= length) return;
+    const int perGroup = p.kvHeads / p.groups, kh0 = g * perGroup, all = perGroup * live;
+    const size_t at = (size_t(b) * p.groups + g) * p.capacity, step = size_t(p.kvHeads) * rows;
+    const int2 span = plan.span[b];
+    const int j = block * 1024 + int(threadIdx.x) * 4, fresh = threadIdx.x;
+    const bool cached = plan.scores && j < length, isNew = block == 0 && fresh < count && length + fresh < p.capacity;
+    float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    float newSum = 0.0f;
+    for (int n0 = 0; n0 < all; n0 += 64) {
+        const int batch = min(64, all - n0);
+        for (int n = wave; n < batch; n += 4) {
+            const int kh = kh0 + (n0 + n) / live, row = (n0 + n) % live;
+            float mx;
+            const float2 st = joinedSum(plan, size_t(span.x) * step + size_t(kh) * rows + row, step, span.y, mx);
+            if (lane == 0) sStat[n] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int n = 0; n < batch; ++n) {
+            const size_t row = (size_t(b) * p.kvHeads + kh0 + (n0 + n) / live) * rows + (n0 + n) % live;
+            const float2 st = sStat[n];
+            if (cached) {
+                const float4v x = loadf4(plan.scores + row * plan.scorePitch + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
+            }
+            if (isNew) newSum += __builtin_amdgcn_exp2f(fmaf(plan.newScores[row * 64 + fresh], plan.c, -st.x)) * st.y;
+        }
+        __syncthreads();
+    }
+    if (cached) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (j + e < length) p.weightsOut[at + j + e] = (p.weightsIn ? p.weightsIn[at + j + e] : 0.0f) + sum[e];
+    }
+    if (isNew) p.weightsOut[at + length + fresh] = newSum;
+}
+
 // The chunks of a row put together.  LPR lanes hold a row's columns, four each, so that a wavefront reads 64 / LPR chunks at
-// once; WPR wavefronts share a row's chunks (one where the sequences have few, four where they have many).
+// once; WPR wavefronts share a row's chunks (one where the sequences have few, four where they have many).  Workgroups
+// past `joinBlocks` make the weights.
 template <int LPR, int WPR>
-__global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan plan) {
+__global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan plan, unsigned joinBlocks) {
     constexpr int CPW = 64 / LPR, STEP = CPW * WPR;
     __shared__ float4v sAcc[4][LPR];
+    if (blockIdx.x >= joinBlocks) {
+        weightsFromScores(p, plan, int(blockIdx.x - joinBlocks));
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = p.heads / p.kvHeads, rows = p.nodes * share;
     const size_t flat = WPR == 4 ? blockIdx.x : size_t(blockIdx.x) * 4 + wave;
     if (flat >= size_t(p.batch) * p.kvHeads * rows) return;
@@ -452,21 +517,13 @@ __global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan pla
     if (row >= nodesInUse(p, b) * share || span.y == 1) return;   // no such row, or written by its only chunk
     const size_t step = size_t(p.kvHeads) * rows, at = size_t(span.x) * step + size_t(kh) * rows + row;
     const int sub = lane % LPR, first = (WPR == 4 ? wave * CPW : 0) + lane / LPR;
-    float most = kNoRef, mx = -INFINITY, sum = 0.0f;
-    for (int c = lane; c < span.y; c += 64) most = fmaxf(most, plan.partStat[at + c * step].x);
-    most = waveMax(most);
-    for (int c = lane; c < span.y; c += 64) {
-        const float4v st = plan.partStat[at + c * step];
-        sum += st.y * __builtin_amdgcn_exp2f(st.x - most);
-        mx = fmaxf(mx, st.z);
-    }
-    sum = waveSum(sum);
-    mx = waveMax(mx);
+    float mx;
+    const float2 total = joinedSum(plan, at, step, span.y, mx);
     float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool on = sub * 4 < p.hd;
 #pragma unroll 4
     for (int c = first; c < span.y; c += STEP) {
-        const float f = __builtin_amdgcn_exp2f(plan.partStat[at + c * step].x - most);
+        const float f = __builtin_amdgcn_exp2f(plan.partStat[at + c * step].x - total.x);
         const float4v x = on ? loadf4(plan.partOut + (at + c * step) * plan.partPitch + sub * 4) : float4v{0.0f, 0.0f, 0.0f, 0.0f};
         acc = acc + x * f;
     }
@@ -480,51 +537,14 @@ __global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan pla
         if (wave != 0) return;
         acc = (sAcc[0][sub] + sAcc[1][sub]) + (sAcc[2][sub] + sAcc[3][sub]);
     }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inv = total.y == 0.0f ? 0.0f : 1.0f / total.y;
     float* dst = p.out + (size_t(b) * p.nodes + row / share) * p.heads * p.hd + size_t(kh * share + row % share) * p.hd + sub * 4;
     if (lane < LPR) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (sub * 4 + j < p.hd) dst[j] = acc[j] * inv;
     }
-    if (lane == 0) finishStats(p, plan, b, kh, row, most, sum, mx);
-}
-
-// The weights from the kept dot products: four keys a thread, the rows of a group one after the other.  The new rows' weights
-// are made by the first workgroup of each (sequence, group).
-__global__ void __launch_bounds__(256) treeWeightsFromScoresKernel(TreeParams p, TilePlan plan) {
-    const int g = blockIdx.y, b = blockIdx.z, share = p.heads / p.kvHeads, rows = p.nodes * share;
-    const int length = rowsInUse(p, b), count = nodesInUse(p, b), live = count * share;
-    const int perGroup = p.kvHeads / p.groups, kh0 = g * perGroup;
-    const size_t at = (size_t(b) * p.groups + g) * p.capacity;
-    const int j = (int(blockIdx.x) * 256 + int(threadIdx.x)) * 4;
-    if (plan.scores && j < length) {
-        float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int kh = kh0; kh < kh0 + perGroup; ++kh) {
-            const size_t first = (size_t(b) * p.kvHeads + kh) * rows;
-#pragma unroll 4
-            for (int row = 0; row < live; ++row) {
-                const float2 st = plan.stat2[first + row];
-                const float4v x = loadf4(plan.scores + (first + row) * plan.scorePitch + j);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (j + e < length) p.weightsOut[at + j + e] = (p.weightsIn ? p.weightsIn[at + j + e] : 0.0f) + sum[e];
-    }
-    if (blockIdx.x == 0 && threadIdx.x < unsigned(count) && length + int(threadIdx.x) < p.capacity) {
-        float sum = 0.0f;
-        for (int kh = kh0; kh < kh0 + perGroup; ++kh) {
-            const size_t first = (size_t(b) * p.kvHeads + kh) * rows;
-            for (int row = 0; row < live; ++row) {
-                const float2 st = plan.stat2[first + row];
-                sum += __builtin_amdgcn_exp2f(fmaf(plan.newScores[(first + row) * 64 + threadIdx.x], plan.c, -st.x)) * st.y;
-            }
-        }
-        p.weightsOut[at + length + threadIdx.x] = sum;
-    }
+    if (lane == 0) finishStats(p, plan, b, kh, row, total.x, total.y, mx);
 }
 
 // ---- the weight of keys from statistics --------------------------------------------------------
@@ -915,18 +935,21 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
 }
 
 template <int LPR>
-int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, hipStream_t s) {
+int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
     // chunks a sequence has on average: four wavefronts a row once one would go round more than four times
-    if (size_t(plan.items) > size_t(p.batch) * 4 * (64 / LPR)) treeJoinKernel<LPR, 4><<<unsigned(rows), 256, 0, s>>>(p, plan);
-    else treeJoinKernel<LPR, 1><<<unsigned((rows + 3) / 4), 256, 0, s>>>(p, plan);
+    const bool many = size_t(plan.items) > size_t(p.batch) * 4 * (64 / LPR);
+    const size_t blocks = size_t(plan.items) == size_t(p.batch) ? 0 : many ? rows : (rows + 3) / 4;   // one chunk each: nothing to join
+    if (blocks + weightBlocks == 0) return BF_OK;
+    if (many) treeJoinKernel<LPR, 4><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
+    else treeJoinKernel<LPR, 1><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
-int launchJoin(const TreeParams& p, const TilePlan& plan, size_t rows, hipStream_t s) {
-    if (p.hd <= 32) return launchJoinOf<8>(p, plan, rows, s);
-    if (p.hd <= 64) return launchJoinOf<16>(p, plan, rows, s);
-    if (p.hd <= 128) return launchJoinOf<32>(p, plan, rows, s);
-    return launchJoinOf<64>(p, plan, rows, s);
+int launchJoin(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
+    if (p.hd <= 32) return launchJoinOf<8>(p, plan, rows, weightBlocks, s);
+    if (p.hd <= 64) return launchJoinOf<16>(p, plan, rows, weightBlocks, s);
+    if (p.hd <= 128) return launchJoinOf<32>(p, plan, rows, weightBlocks, s);
+    return launchJoinOf<64>(p, plan, rows, weightBlocks, s);
 }
 
 int checkHeads(const char* fn, size_t heads, size_t kvHeads, size_t groups, size_t headDim) {
@@ -950,7 +973,6 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
         return failInvalid(fn, "NULL pointer");
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.nodes = int(nodes);
     p.capacity = int(capacity); p.hd = int(headDim);
-    hipStream_t s = asStream(stream);
     const size_t share = heads / kvHeads, rows = nodes * share;
     const bool keepScores = weights && capacity != 0 && rows <= 16;
     const bool recompute = weights && capacity != 0 && !keepScores;
@@ -972,11 +994,16 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     plan.partPitch = int((headDim + 3) / 4 * 4);
     const bool join = size_t(plan.items) > batch;
     const size_t slots = size_t(plan.items) * kvHeads * rows, rowsAll = batch * kvHeads * rows;
-    const size_t need[] = {join ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
+    plan.keyBlocks = keepScores ? std::max(1, int((capacity + 1023) / 1024)) : 1;
+    const size_t weightBlocks = weights && capacity != 0 ? batch * groups * size_t(plan.keyBlocks) : 0;
+    if (rowsAll + weightBlocks >= (size_t(1) << 31) || size_t(plan.items) * kvHeads * size_t(plan.rowGroups) >= (size_t(1) << 31))
+        return failInvalid(fn, "shape too large");
+    const size_t need[] = {join || weights ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
                            keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, weights ? rowsAll * 64 * sizeof(float) : 0,
-                           weights ? rowsAll * sizeof(float2) : 0, recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
-    size_t bytes = 0, offset[7];
-    for (int i = 0; i < 7; ++i) {
+                           recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
+    hipStream_t s = asStream(stream);
+    size_t bytes = 0, offset[6];
+    for (int i = 0; i < 6; ++i) {
         offset[i] = bytes;
         bytes += (need[i] + 255) / 256 * 256;
     }
@@ -988,8 +1015,7 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     plan.span = reinterpret_cast<int2*>(part(2));
     plan.scores = reinterpret_cast<float*>(part(3));
     plan.newScores = reinterpret_cast<float*>(part(4));
-    plan.stat2 = reinterpret_cast<float2*>(part(5));
-    if (float* own2 = reinterpret_cast<float*>(part(6))) {
+    if (float* own2 = reinterpret_cast<float*>(part(5))) {
         if (!p.m) p.m = own2;
         if (!p.l) p.l = own2 + rowsAll;
     }
@@ -997,15 +1023,9 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const int mode = headDim % 4 != 0 || !aligned16({p.q, p.kNew, p.vNew, p.k, p.v, p.out}) ? 0 : headDim == size_t(hdp) ? 2 : 1;
     st = launchTiles(p, plan, hdp, rt, mode, grid, s);
     if (st != BF_OK) return st;
-    if (join) {
-        st = launchJoin(p, plan, rowsAll, s);
-        if (st != BF_OK) return st;
-    }
-    if (weights && capacity != 0) {
-        // the new rows' weights, and the cached rows' where their dot products were kept
-        treeWeightsFromScoresKernel<<<dim3(keepScores ? unsigned((capacity + 1023) / 1024) : 1u, unsigned(groups), unsigned(batch)), 256, 0, s>>>(p, plan);
-        BF_LAUNCH_CHECK();
-    }
+    // the new rows' weights, and the cached rows' where their dot products were kept, ride on the launch that joins
+    st = launchJoin(p, plan, rowsAll, weightBlocks, s);
+    if (st != BF_OK) return st;
     if (recompute) {
         KeyWeightParams w{};
         w.q = p.q; w.k = p.k; w.m = p.m; w.l = p.l; w.counts = p.counts; w.lengths = p.lengths; w.weightsIn = p.weightsIn; w.weightsOut = p.weightsOut;
