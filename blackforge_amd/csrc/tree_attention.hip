@@ -436,20 +436,26 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     }
 }
 
-// A row's reference and sum over its chunks, by a wavefront; `at` + c * `step` is chunk c's entry
+// A row's reference and sum over its chunks, by LANES neighbouring lanes; `at` + c * `step` is chunk c's entry
+template <int LANES>
 __device__ __forceinline__ float2 joinedSum(const TilePlan& plan, size_t at, size_t step, int chunks, float& mx) {
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x % LANES;
     float most = kNoRef, sum = 0.0f;
-    for (int c = lane; c < chunks; c += 64) most = fmaxf(most, plan.partStat[at + c * step].x);
-    most = waveMax(most);
+    for (int c = lane; c < chunks; c += LANES) most = fmaxf(most, plan.partStat[at + c * step].x);
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, 64));
     mx = -INFINITY;
-    for (int c = lane; c < chunks; c += 64) {
+    for (int c = lane; c < chunks; c += LANES) {
         const float4v st = plan.partStat[at + c * step];
         sum += st.y * __builtin_amdgcn_exp2f(st.x - most);
         mx = fmaxf(mx, st.z);
     }
-    mx = waveMax(mx);
-    return make_float2(most, waveSum(sum));
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) {
+        sum += __shfl_xor(sum, off, 64);
+        mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+    }
+    return make_float2(most, sum);
 }
 
 // The weights of a block of 1024 cached rows, four a thread, from the kept dot products of the group's rows; the block of
@@ -473,7 +479,7 @@ __device__ __forceinline__ void weightsFromScores(const TreeParams& p, const Til
         for (int n = wave; n < batch; n += 4) {
             const int kh = kh0 + (n0 + n) / live, row = (n0 + n) % live;
             float mx;
-            const float2 st = joinedSum(plan, size_t(span.x) * step + size_t(kh) * rows + row, step, span.y, mx);
+            const float2 st = joinedSum<64>(plan, size_t(span.x) * step + size_t(kh) * rows + row, step, span.y, mx);
             if (lane == 0) sStat[n] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
         }
         __syncthreads();
@@ -498,53 +504,51 @@ __device__ __forceinline__ void weightsFromScores(const TreeParams& p, const Til
     if (isNew) p.weightsOut[at + length + fresh] = newSum;
 }
 
-// The chunks of a row put together.  LPR lanes hold a row's columns, four each, so that a wavefront reads 64 / LPR chunks at
-// once; WPR wavefronts share a row's chunks (one where the sequences have few, four where they have many).  Workgroups
-// past `joinBlocks` make the weights.
-template <int LPR, int WPR>
+// The chunks of a row put together.  LPR lanes hold a row's columns, four each.  Few chunks a row (MANY false): every LPR
+// lanes have a row of their own and take its chunks in turn, so that few wavefronts wait out the chain of loads (24000 rows
+// of three chunks: 15 us with a wavefront each).  Many: a workgroup a row, 256 / LPR chunks at once.  Workgroups past
+// `joinBlocks` make the weights.
+template <int LPR, bool MANY>
 __global__ void __launch_bounds__(256) treeJoinKernel(TreeParams p, TilePlan plan, unsigned joinBlocks) {
-    constexpr int CPW = 64 / LPR, STEP = CPW * WPR;
+    constexpr int STEP = MANY ? 256 / LPR : 1;
     __shared__ float4v sAcc[4][LPR];
     if (blockIdx.x >= joinBlocks) {
         weightsFromScores(p, plan, int(blockIdx.x - joinBlocks));
         return;
     }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = p.heads / p.kvHeads, rows = p.nodes * share;
-    const size_t flat = WPR == 4 ? blockIdx.x : size_t(blockIdx.x) * 4 + wave;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, share = p.heads / p.kvHeads, rows = p.nodes * share, sub = lane % LPR;
+    const size_t flat = MANY ? blockIdx.x : size_t(blockIdx.x) * (256 / LPR) + threadIdx.x / LPR;
     if (flat >= size_t(p.batch) * p.kvHeads * rows) return;
     const int row = int(flat % rows), kh = int(flat / rows % p.kvHeads), b = int(flat / rows / p.kvHeads);
     const int2 span = plan.span[b];
     if (row >= nodesInUse(p, b) * share || span.y == 1) return;   // no such row, or written by its only chunk
     const size_t step = size_t(p.kvHeads) * rows, at = size_t(span.x) * step + size_t(kh) * rows + row;
-    const int sub = lane % LPR, first = (WPR == 4 ? wave * CPW : 0) + lane / LPR;
     float mx;
-    const float2 total = joinedSum(plan, at, step, span.y, mx);
+    const float2 total = joinedSum<MANY ? 64 : LPR>(plan, at, step, span.y, mx);
     float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool on = sub * 4 < p.hd;
 #pragma unroll 4
-    for (int c = first; c < span.y; c += STEP) {
+    for (int c = MANY ? int(threadIdx.x) / LPR : 0; c < span.y; c += STEP) {
         const float f = __builtin_amdgcn_exp2f(plan.partStat[at + c * step].x - total.x);
         const float4v x = on ? loadf4(plan.partOut + (at + c * step) * plan.partPitch + sub * 4) : float4v{0.0f, 0.0f, 0.0f, 0.0f};
         acc = acc + x * f;
     }
+    if constexpr (MANY) {
 #pragma unroll
-    for (int off = LPR; off < 64; off <<= 1)
+        for (int off = LPR; off < 64; off <<= 1)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], off, 64);
-    if constexpr (WPR == 4) {
+            for (int j = 0; j < 4; ++j) acc[j] += __shfl_xor(acc[j], off, 64);
         if (lane < LPR) sAcc[wave][lane] = acc;
         __syncthreads();
-        if (wave != 0) return;
+        if (threadIdx.x >= LPR) return;
         acc = (sAcc[0][sub] + sAcc[1][sub]) + (sAcc[2][sub] + sAcc[3][sub]);
     }
     const float inv = total.y == 0.0f ? 0.0f : 1.0f / total.y;
     float* dst = p.out + (size_t(b) * p.nodes + row / share) * p.heads * p.hd + size_t(kh * share + row % share) * p.hd + sub * 4;
-    if (lane < LPR) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (sub * 4 + j < p.hd) dst[j] = acc[j] * inv;
-    }
-    if (lane == 0) finishStats(p, plan, b, kh, row, total.x, total.y, mx);
+    for (int j = 0; j < 4; ++j)
+        if (sub * 4 + j < p.hd) dst[j] = acc[j] * inv;
+    if (sub == 0) finishStats(p, plan, b, kh, row, total.x, total.y, mx);
 }
 
 // ---- the weight of keys from statistics --------------------------------------------------------
@@ -936,12 +940,12 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
 
 template <int LPR>
 int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
-    // chunks a sequence has on average: four wavefronts a row once one would go round more than four times
-    const bool many = size_t(plan.items) > size_t(p.batch) * 4 * (64 / LPR);
-    const size_t blocks = size_t(plan.items) == size_t(p.batch) ? 0 : many ? rows : (rows + 3) / 4;   // one chunk each: nothing to join
+    // few chunks a row on average, unless there are so few rows that their lanes would not fill the device
+    const bool many = size_t(plan.items) > size_t(p.batch) * (rows * LPR > size_t(computeUnits()) * 512 ? 32 : 4);
+    const size_t blocks = size_t(plan.items) == size_t(p.batch) ? 0 : many ? rows : (rows * LPR + 255) / 256;   // one chunk each: nothing to join
     if (blocks + weightBlocks == 0) return BF_OK;
-    if (many) treeJoinKernel<LPR, 4><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
-    else treeJoinKernel<LPR, 1><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
+    if (many) treeJoinKernel<LPR, true><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
+    else treeJoinKernel<LPR, false><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
