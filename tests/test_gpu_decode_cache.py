@@ -6,6 +6,8 @@ ds = (headDim + 4) e scale max(|q| . |k|), including the rounding of its scaling
 relative to itself (N visible keys in the sum), and a weighted mean of values by twice that times max|v|, N e max|v| included.
 """
 import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -686,3 +688,11 @@ def test_caches_past_two_to_the_32_elements(hip, rng):
     assert dl.toHostInts().tolist() == [0] * (batch - 1) + [300]
     del k, v
     call("bf_hip_pool_trim")
+
+
+def test_the_cpp_layer(hip):
+    """tests/cpp/decode_cache_test.cpp: the same operators through namespace blackforge::backend::hip."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "blackforge_amd", "host", "bin", "decode_cache_test")
+    assert os.path.exists(exe), "blackforge_amd/host has not been built"
+    proc = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert proc.returncode == 0, proc.stdout + proc.stderr
