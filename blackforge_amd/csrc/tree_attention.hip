@@ -54,6 +54,7 @@ __device__ __forceinline__ unsigned long long newRowsSeen(const TreeParams& p, i
 struct TilePlan {
     int target;          // chunks per (key head, group of row tiles) that the launch wants in total over the sequences
     int minChunk;        // keys a chunk has at least
+    float slots;         // chunks (per key head and group of row tiles) that run at once; 0: even shares of `target`
     int items;           // workgroups along the sequences' chunks: at least the number of chunks there will be
     int rowGroups;       // groups of RT row tiles
     float4v* partStat;   // [item][kvHeads][rows]: ref, l, largest dot product
@@ -65,28 +66,62 @@ struct TilePlan {
     float c;             // |scale| log2(e)
 };
 
-// Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for
-// each.  Returns this item's sequence (-1: there is none) and its chunk.
+// Where the products bound the pass, what a chunk size costs is the number of rounds its workgroups take on the device's
+// slots times the length of a round, and neighbouring sizes differ much (32 equal sequences, 12 heads, 512 slots: three
+// chunks each are 1152 workgroups, 3 rounds of a third; four are 1536, 3 rounds of a quarter).  Lane c of the wavefront tries one
+// size, from half as much again as fills the slots once down to a third of it; the cheapest is taken, the larger on a tie.
+__device__ __forceinline__ int bestChunk(const TreeParams& p, const TilePlan& plan, int length, int total) {
+    const int lane = threadIdx.x & 63, mine = (length + 63) / 64;
+    const float base = float(total) / plan.slots;            // units of 64 keys that fill the slots once
+    const int least = plan.minChunk / 64;
+    const float size = fmaxf(float(least), ceilf(base * 1.5f * 18.0f / (18.0f + float(lane))));
+    const float over = 1.0f / size;
+    float chunks = 0.0f;
+    for (int b = 0; b < p.batch; ++b) chunks += fmaxf(1.0f, ceilf(float(__builtin_amdgcn_readlane(mine, b)) * over - 1e-4f));
+    float cost = ceilf(chunks / plan.slots - 1e-4f) * (size + 2.0f);   // 2: what a chunk costs beside its keys
+    if (chunks > float(plan.target)) cost = INFINITY;        // more than there will be workgroups
+    int best = int(size);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const float otherCost = __shfl_xor(cost, off, 64);
+        const int other = __shfl_xor(best, off, 64);
+        if (otherCost < cost || (otherCost == cost && other > best)) { cost = otherCost; best = other; }
+    }
+    return cost == INFINITY ? int(ceilf(base * 2.0f)) + 1 : best;
+}
+
+// Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for each (a
+// sequence without nodes has nothing to read).  Returns this item's sequence (-1: there is none) and its chunk.
 struct Chunk { int b, first, count, start, end, queries; };
 __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& plan, int item) {
     const int lane = threadIdx.x & 63;
-    const int length0 = lane < p.batch ? rowsInUse(p, lane) : 0, count0 = lane < p.batch ? nodesInUse(p, lane) : 0;
+    auto sequence = [&](int b, int& rows, int& nodes) {
+        nodes = b < p.batch ? nodesInUse(p, b) : 0;
+        rows = nodes > 0 ? rowsInUse(p, b) : 0;
+    };
+    int length0, count0;
+    sequence(lane, length0, count0);
     long long total = (length0 + 63) / 64;   // in units of 64 rows
-    for (int b0 = 64; b0 < p.batch; b0 += 64) total += b0 + lane < p.batch ? (rowsInUse(p, b0 + lane) + 63) / 64 : 0;
+    for (int b0 = 64; b0 < p.batch; b0 += 64) {
+        int length, count;
+        sequence(b0 + lane, length, count);
+        total += (length + 63) / 64;
+    }
     if (p.batch > 1) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
     } else {
         total = __shfl(total, 0, 64);
     }
-    const int even = int(min((total + plan.target - 1) / plan.target, (long long)(1 << 24)));
-    const int size = max(plan.minChunk, even * 64);
+    int units = int(min((total + plan.target - 1) / plan.target, (long long)(1 << 24)));
+    if (plan.slots > 0 && p.batch <= 64) units = bestChunk(p, plan, length0, int(total));
+    const int size = max(plan.minChunk, units * 64);
     Chunk c{-1, 0, 0, 0, 0, 0};
     int before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
         const bool on = b0 + lane < p.batch;
-        const int length = b0 == 0 ? length0 : on ? rowsInUse(p, b0 + lane) : 0;
-        const int count = b0 == 0 ? count0 : on ? nodesInUse(p, b0 + lane) : 0;
+        int length = length0, count = count0;
+        if (b0 != 0) sequence(b0 + lane, length, count);
         const int mine = on ? max(1, (length + size - 1) / size) : 0;
         int upTo = mine;
         if (p.batch > 1) {
@@ -987,10 +1022,19 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     TilePlan plan{};
     plan.rowGroups = int((rows + 16 * rt - 1) / (16 * rt));
     plan.minChunk = 128;
-    // Workgroups a compute unit gets: eight where a wavefront holds one row tile (its partial results are small: 16 ragged
-    // sequences of up to 16000 rows 400 us with four, 376 with eight), four otherwise (64 nodes over 32 ragged sequences
-    // 173 / 160 / 166 us with two, four, eight; 16 nodes of four heads each 142 / 111 / 130).
-    plan.target = int(std::max<size_t>(1, size_t(computeUnits()) * (rt == 1 ? 8 : 4) / (kvHeads * size_t(plan.rowGroups))));
+    // One row tile: the pass is a stream, and eight workgroups a compute unit in even shares keep it full (16 ragged sequences of
+    // up to 16000 rows: 400 us with four, 376 with eight).  More: chunk sizes by the rounds they make (bestChunk), with the
+    // workgroups whose registers a compute unit holds; even shares of four a compute unit measured 337 us where that gives 327
+    // (26 nodes over 120011 rows) and 160 where it gives 151 (50000 rows), and the other way round 112 and 114 us (16 nodes of
+    // four heads each over 8 ragged sequences).
+    const size_t device = size_t(computeUnits()), pairs = kvHeads * size_t(plan.rowGroups);
+    if (rt == 1) {
+        plan.target = int(std::max<size_t>(1, device * 8 / pairs));
+    } else {
+        plan.slots = float(device * (hdp * rt <= 128 ? 3 : 2)) / float(pairs);
+        plan.target = int(std::max<size_t>(1, size_t(3.0f * plan.slots + 0.5f))) + int(batch);
+    }
+    // Even shares are at most target + batch chunks, and so are those of bestChunk, whose own count may miss one a sequence
     const size_t chunksAtMost = batch * std::max<size_t>(1, (capacity + plan.minChunk - 1) / plan.minChunk);
     plan.items = int(std::min(chunksAtMost, size_t(plan.target) + batch));
     plan.c = float(std::fabs(double(p.scale)) * 1.4426950408889634074);

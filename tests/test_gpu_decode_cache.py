@@ -142,6 +142,9 @@ TREES = [
     (1, 4, 2, 252, 64, 90, [77], [64]),
     (1, 2, 2, 64, 8, 20000, [19999], [8]),
     (5, 16, 16, 128, 3, 3000, [2999, 0, 1024, 5, 2048], [3, 3, 1, 2, 3]),
+    (12, 2, 2, 64, 20, 3000, [3000] * 12, [0] * 11 + [20]),                       # sequences without nodes, with long caches
+    (9, 3, 3, 64, 40, 2100, [2100, 64, 0, 2099, 700, 1, 1337, 63, 65], [40, 33, 40, 1, 17, 40, 0, 40, 16]),
+    (66, 4, 2, 128, 12, 400, [(61 * i) % 401 for i in range(66)], [(5 * i) % 13 for i in range(66)]),
     (70, 2, 2, 64, 2, 50, [(7 * i) % 51 for i in range(70)], [i % 3 for i in range(70)]),
 ]
 
