@@ -64,6 +64,7 @@ struct TilePlan {
     float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
     int scorePitch, partPitch, keyBlocks;
     float c;             // |scale| log2(e)
+    unsigned magic;      // 2^32 / (heads / kvHeads), rounded up
 };
 
 // Where the products bound the pass, what a chunk size costs is the number of rounds its workgroups take on the device's
@@ -181,6 +182,9 @@ __device__ __forceinline__ void finishStats(const TreeParams& p, const TilePlan&
 constexpr float kNoRef = -3.402823466e38f;   // a reference below every score: the first real one moves it
 constexpr float kRefSlack = 8.0f;
 
+// The node of a row and its head among the heads that share its key head; `magic` is 2^32 / share rounded up
+__device__ __forceinline__ int nodeOf(const TilePlan& plan, int share, int row) { return share == 1 ? row : int(__umulhi(unsigned(row), plan.magic)); }
+
 // wavefronts per SIMD that the registers of a form allow
 constexpr int tileWaves(int hdp, int rt) { return hdp * rt <= 64 ? 3 : hdp * rt <= 256 && hdp <= 128 ? 2 : 1; }
 template <int HDP, int RT, int MODE, bool SCORES>
@@ -188,12 +192,11 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     constexpr int KS = HDP / 16;                    // 16-column steps of the dot products
     constexpr int VW = HDP >= 64 ? 4 : 2;           // value columns a lane loads at once
     constexpr int VU = HDP / (16 * VW);             // such loads
-    extern __shared__ float smem[];
+    constexpr int PITCH = HDP + 4;
+    extern __shared__ float smem[];                 // [wavefront][row][PITCH]: the outputs to be joined
     __shared__ float4v sStat[4][RT * 16];
     __shared__ unsigned sOdd[4];   // new rows of each 16 that hold a value which is not finite
-    if (threadIdx.x < 4) sOdd[threadIdx.x] = 0;
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, g = lane >> 4;
     // the row groups of one chunk next to each other on one XCD (workgroups go to the 8 XCDs in turn), where they share its reads
     const unsigned perXcd = blockIdx.x / 8, flat = perXcd / plan.rowGroups * 8 + blockIdx.x % 8;
     const int rowGroup = perXcd % plan.rowGroups;
@@ -207,29 +210,48 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     const int row0 = rowGroup * RT * 16;
     if (row0 >= live) return;
     const int tiles = min(RT, (live - row0 + 15) / 16);
-    const size_t kvDim = size_t(p.kvHeads) * hd;
-    const float* kb = p.k + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
-    const float* vb = p.v + size_t(b) * p.capacity * kvDim + size_t(kh) * hd;
+    const unsigned kvDim = unsigned(p.kvHeads) * hd;
+    if (threadIdx.x < 4) sOdd[threadIdx.x] = 0;
+    __syncthreads();
 
-    // With the sequence's last chunk go its new rows, 16 to a wavefront, starting with the one that has the fewest cached ones
+    // The wavefront's tiles of 16 keys: every fourth of the chunk's, and with the sequence's last chunk 16 of the new rows,
+    // starting with the wavefront that has the fewest cached ones.
+    const int from = ch.start + wave * 16, cachedTiles = max(0, (ch.end - from + 63) / 64);
     const int newTile = (wave - (ch.end - ch.start + 15) / 16) & 3;
     const bool hasNew = item == ch.first + ch.count - 1 && newTile * 16 < count;
+    const size_t firstCached = (size_t(b) * p.capacity + from) * kvDim + size_t(kh) * hd;
+    const size_t firstNew = (size_t(b) * p.nodes + newTile * 16) * kvDim + size_t(kh) * hd;
+    float k[KS][4], v[VU][4][VW];
+    // a tile from its first row, of which rows 0 .. last exist; the addresses are a uniform base and a 32-bit offset
+    auto loadK = [&](const float* base, int last) {
+        const float* src = reinterpret_cast<const float*>(reinterpret_cast<const char*>(base) + 4u * (__umul24(unsigned(min(i16, last)), kvDim) + 4 * g));
+#pragma unroll
+        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(k[s], src - 4 * g, 16 * s + 4 * g, hd);
+    };
+    auto loadV = [&](const float* base, int last) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float* src = reinterpret_cast<const float*>(reinterpret_cast<const char*>(base) + 4u * __umul24(unsigned(min(4 * g + r, last)), kvDim));
+#pragma unroll
+            for (int u = 0; u < VU; ++u) loadColumns<MODE, VW>(v[u][r], src, u * 16 * VW + i16 * VW, hd);
+        }
+    };
     unsigned seen[RT];   // bits 0..3: new rows 16 newTile + 4 g .. that this lane's row of tile t sees
-
     float q[RT][KS][4];
     const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+    const float* qBase = p.q + size_t(b) * p.nodes * p.heads * hd + size_t(kh) * share * hd;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         const int row = row0 + t * 16 + i16;
         const bool on = row < live;
-        const int node = on ? row / share : 0, h = kh * share + (on ? row % share : 0);
-        const float* src = p.q + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd;
+        const int node = on ? nodeOf(plan, share, row) : 0, h = on ? row - node * share : 0;
+        const float* src = qBase + unsigned(node * p.heads + h) * unsigned(hd);
         seen[t] = hasNew && on ? unsigned(newRowsSeen(p, b, node, count) >> (newTile * 16 + 4 * g)) & 15u : 0u;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             loadColumns<MODE, 4>(q[t][s], src, 16 * s + 4 * g, hd);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) q[t][s][c] = on ? q[t][s][c] * sign : 0.0f;
+            for (int c = 0; c < 4; ++c) q[t][s][c] *= on ? sign : 0.0f;
         }
     }
     float4v o[RT][VU][VW];
@@ -242,22 +264,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
 #pragma unroll
             for (int w = 0; w < VW; ++w) o[t][u][w] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
-    float k[KS][4], v[VU][4][VW];
-    // key i16 of 16 from `row`; `last`: the last row that may be read
-    auto loadK = [&](const float* base, int row, int last) {
-        const float* src = base + size_t(min(row + i16, last)) * kvDim;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(k[s], src, 16 * s + 4 * g, hd);
-    };
-    auto loadV = [&](const float* base, int row, int last) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float* src = base + size_t(min(row + 4 * g + r, last)) * kvDim;
-#pragma unroll
-            for (int u = 0; u < VU; ++u) loadColumns<MODE, VW>(v[u][r], src, u * 16 * VW + i16 * VW, hd);
-        }
-    };
+    const int newLast = min(15, count - 1 - newTile * 16);
     auto dotProducts = [&](int t) {
         float4v even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;   // two chains: half the error, and none waits for the one before
 #pragma unroll
@@ -315,16 +322,22 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
                 for (int w = 0; w < VW; ++w) o[t][u][w] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[u][r][w], x[r], o[t][u][w], 0, 0, 0);
     };
 
-    // Cached rows: the four wavefronts take 16 keys in turn.  The body is straight-line code for the number of row tiles in
-    // use, and no load in it stands behind a branch (the waits for the loads before it would have to assume the worst).
+    // The cached tiles.  The body is straight-line code for the number of row tiles in use, and no load in it stands behind a
+    // branch (the waits for the loads before it would have to assume the worst); the last tile fetches the new rows'.
     auto walk = [&](auto tileCount) {
         constexpr int N = decltype(tileCount)::value;
-        const int last = ch.end - 1;
-        int key = ch.start + wave * 16;
-        if (key >= ch.end) return;
-        loadK(kb, key, last);
-        loadV(vb, key, last);
-        for (; key < ch.end; key += 64) {
+        if (cachedTiles + int(hasNew) == 0) return;
+        const float* kAt = cachedTiles > 0 ? p.k + firstCached : p.kNew + firstNew;
+        const float* vAt = cachedTiles > 0 ? p.v + firstCached : p.vNew + firstNew;
+        const int lastAt = cachedTiles > 0 ? min(15, ch.end - 1 - from) : newLast;
+        loadK(kAt, lastAt);
+        loadV(vAt, lastAt);
+        for (int n = 0; n < cachedTiles; ++n) {
+            const int key = from + n * 64;
+            const bool more = n + 1 < cachedTiles;
+            const float* kNext = more ? kAt + size_t(64) * kvDim : hasNew ? p.kNew + firstNew : kAt;
+            const float* vNext = more ? vAt + size_t(64) * kvDim : hasNew ? p.vNew + firstNew : vAt;
+            const int lastNext = more ? min(15, ch.end - 1 - key - 64) : hasNew ? newLast : 0;
             float x[RT][4];
 #pragma unroll
             for (int t = 0; t < N; ++t) {
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x[t][r] = dots[r];
             }
-            loadK(kb, key + 64, last);   // past the end: the last row again
+            loadK(kNext, lastNext);
             if (key + 16 > ch.end) {     // values of keys past the end: whatever lies there must not meet a weight of zero
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -355,7 +368,39 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
             probabilities(tileCount, x);
 #pragma unroll
             for (int t = 0; t < N; ++t) addValues(t, x[t]);
-            loadV(vb, key + 64, last);
+            loadV(vNext, lastNext);
+            kAt = kNext;
+            vAt = vNext;
+        }
+        if (hasNew) {
+            const int j0 = newTile * 16;
+            // A value that is not finite must not meet the weight zero of a row that does not see it: taken out here, added to
+            // the rows that do when the results are written.
+            unsigned notFinite = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int u = 0; u < VU; ++u)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        const bool in = j0 + 4 * g + r < count, finite = fabsf(v[u][r][w]) < INFINITY;
+                        if (in && !finite) notFinite |= 1u << (4 * g + r);
+                        v[u][r][w] = in && finite ? v[u][r][w] : 0.0f;
+                    }
+            if (notFinite) atomicOr(&sOdd[newTile], notFinite);
+            float x[RT][4];
+#pragma unroll
+            for (int t = 0; t < N; ++t) {
+                const float4v dots = dotProducts(t);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[t][r] = seen[t] >> r & 1 ? dots[r] : -INFINITY;
+                const int row = row0 + t * 16 + i16;
+                if (plan.newScores && row < live)
+                    storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
+            }
+            probabilities(tileCount, x);
+#pragma unroll
+            for (int t = 0; t < N; ++t) addValues(t, x[t]);
         }
     };
     if (tiles == RT) walk(std::integral_constant<int, RT>{});
@@ -364,42 +409,8 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         if (tiles == 2) walk(std::integral_constant<int, 2>{});
         if (tiles == 3) walk(std::integral_constant<int, 3>{});
     }
-    if (hasNew) {
-        const int j0 = newTile * 16;
-        const size_t at = size_t(b) * p.nodes * kvDim + size_t(kh) * hd;
-        loadK(p.kNew + at, j0, count - 1);
-        loadV(p.vNew + at, j0, count - 1);
-        // A value that is not finite must not meet the weight zero of a row that does not see it: taken out here, added to
-        // the rows that do when the results are written.
-        unsigned notFinite = 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int u = 0; u < VU; ++u)
-#pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    const bool in = j0 + 4 * g + r < count, finite = fabsf(v[u][r][w]) < INFINITY;
-                    if (in && !finite) notFinite |= 1u << (4 * g + r);
-                    v[u][r][w] = in && finite ? v[u][r][w] : 0.0f;
-                }
-        if (notFinite) atomicOr(&sOdd[newTile], notFinite);
-        float x[RT][4];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const float4v dots = dotProducts(t);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[t][r] = seen[t] >> r & 1 ? dots[r] : -INFINITY;
-            const int row = row0 + t * 16 + i16;
-            if (plan.newScores && row < live)
-                storef4(plan.newScores + ((size_t(b) * p.kvHeads + kh) * rows + row) * 64 + j0 + 4 * g, float4v{x[t][0], x[t][1], x[t][2], x[t][3]});
-        }
-        probabilities(std::integral_constant<int, RT>{}, x);
-#pragma unroll
-        for (int t = 0; t < RT; ++t) addValues(t, x[t]);
-    }
 
-    // the four wavefronts' states joined through LDS, [wave][row][HDP + 4]
-    constexpr int PITCH = HDP + 4;
+    // the four wavefronts' states joined through LDS
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
         if (t < tiles) {
@@ -424,6 +435,8 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     const bool only = ch.count == 1;
     const unsigned long long odd = (unsigned long long)(sOdd[0] | sOdd[1] << 16) | (unsigned long long)(sOdd[2] | sOdd[3] << 16) << 32;
     const int liveHere = min(live - row0, tiles * 16);
+    const size_t entry = (size_t(item) * p.kvHeads + kh) * rows;
+    float* outBase = only ? p.out + size_t(b) * p.nodes * p.heads * hd + size_t(kh) * share * hd : plan.partOut + entry * plan.partPitch;
     // sixteen threads a row, four columns at a time
     for (int e = threadIdx.x; e < liveHere * 16; e += 256) {
         const int r = e >> 4, part = e & 15, row = row0 + r;
@@ -441,15 +454,17 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
             f[w] = __builtin_amdgcn_exp2f(st[w].x - most);
             sum += st[w].y * f[w];
         }
-        const int node = row / share, h = kh * share + row % share;
-        const float inv = only ? (sum == 0.0f ? 0.0f : 1.0f / sum) : 1.0f;
-        float* dst = only ? p.out + (size_t(b) * p.nodes + node) * p.heads * hd + size_t(h) * hd
-                          : plan.partOut + ((size_t(item) * p.kvHeads + kh) * rows + row) * plan.partPitch;
+        const int node = nodeOf(plan, share, row), h = row - node * share;
+        if (only) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) f[w] *= inv;
+        }
+        float* dst = outBase + (only ? unsigned(node * p.heads + h) * unsigned(hd) : unsigned(row) * unsigned(plan.partPitch));
         for (int d = part * 4; d < hd; d += 64) {
             float4v acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int w = 0; w < 4; ++w) acc = acc + *reinterpret_cast<const float4v*>(smem + (w * RT * 16 + r) * PITCH + d) * f[w];
-            acc = acc * inv;
             if (odd != 0) {
                 for (unsigned long long left = odd & newRowsSeen(p, b, node, count); left != 0; left &= left - 1) {
                     const float* src = p.vNew + (size_t(b) * p.nodes + __ffsll(left) - 1) * kvDim + size_t(kh) * hd + d;
@@ -466,7 +481,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
         }
         if (part == 0) {
             if (only) finishStats(p, plan, b, kh, row, most, sum, mx);
-            if (plan.partStat) plan.partStat[(size_t(item) * p.kvHeads + kh) * rows + row] = float4v{most, sum, mx, 0.0f};
+            if (plan.partStat) plan.partStat[entry + row] = float4v{most, sum, mx, 0.0f};
         }
     }
 }
@@ -1038,6 +1053,7 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const size_t chunksAtMost = batch * std::max<size_t>(1, (capacity + plan.minChunk - 1) / plan.minChunk);
     plan.items = int(std::min(chunksAtMost, size_t(plan.target) + batch));
     plan.c = float(std::fabs(double(p.scale)) * 1.4426950408889634074);
+    plan.magic = unsigned(((size_t(1) << 32) + share - 1) / share);
     plan.scorePitch = int((capacity + 15) / 16 * 16);
     plan.partPitch = int((headDim + 3) / 4 * 4);
     const bool join = size_t(plan.items) > batch;
