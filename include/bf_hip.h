@@ -477,7 +477,8 @@ int bf_hip_counter_add(int* counter, int by, bf_stream_t stream);
  * [batch, heads, nodes], the statistics of attention_forward (maximum of the scaled scores and sum of exp(score - m)),
  * each may be NULL.  A node that sees nothing, or nothing but scores of -infinity, gets out = 0, l = 0 (m = -infinity).
  * Nodes i >= counts[b] are neither read nor written, and neither are rows that a node does not see: what lies there may
- * be NaN.  Any alignment; 16-byte aligned operands with headDim a multiple of 4 are faster. */
+ * be NaN; a value that is not finite makes the outputs of the nodes that see it not finite.  Any alignment; 16-byte
+ * aligned operands with headDim a multiple of 4 are faster. */
 int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
                           const int* counts, const uint64_t* visible, float* out, float* m, float* l, size_t batch, size_t heads, size_t kvHeads,
                           size_t nodes, size_t capacity, size_t headDim, float scale, bf_stream_t stream);
@@ -495,7 +496,8 @@ int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float
  * that attention_forward left for q [batch, newLen, heads * headDim] and the keys k [batch, kvRows, kvHeads * headDim],
  * weightsOut[b, g, j] = weightsIn[b, g, j] + sum over the heads of group g and the queries i < counts[b] (NULL: newLen)
  * with j <= oldLen + i of exp(score_ij - m_i) / l_i, for j < totalLen; weights: [batch, groups, weightRows].  A row with
- * l = 0 gives nothing.  weightsIn may be NULL (zeros) or weightsOut itself.  oldLen >= totalLen - 1: no causal mask. */
+ * l = 0 gives nothing.  weightsIn may be NULL (zeros) or weightsOut itself.  oldLen >= totalLen - 1: no causal mask.
+ * The q and k that count must be finite: past 64 queries the products are made of bf16 terms, which infinities have none. */
 int bf_hip_attention_key_weights(const float* q, const float* k, const float* m, const float* l, const int* counts, const float* weightsIn,
                                  float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t newLen, size_t totalLen,
                                  size_t kvRows, size_t headDim, float scale, size_t oldLen, size_t weightRows, bf_stream_t stream);
