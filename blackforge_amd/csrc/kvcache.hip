@@ -343,9 +343,8 @@ __global__ void __launch_bounds__(256) kvCommitKernel(CommitParams p) {
         const int node = lane < count ? p.path[size_t(b) * p.nodes + lane] : 0;
         for (int g = 0; g < p.groups; ++g) {
             float* w = p.weights[layer] + (size_t(b) * p.groups + g) * p.capacity + length;
-            const bool live = lane < count && length + node < p.capacity;
-            const float x = live ? w[node] : 0.0f;
-            if (live) w[lane] = x;
+            const float x = lane < count && length + node < p.capacity ? w[node] : 0.0f;   // past the capacity none was kept
+            if (lane < count) w[lane] = x;
         }
     }
 }

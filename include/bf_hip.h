@@ -524,7 +524,8 @@ int bf_hip_tree_accept(const float* logits, const float* tokens, const int* pare
 /* The accepted nodes' keys and values appended to the caches of all layers: row path[b, i] of kNew, vNew (of every layer,
  * [batch, nodes, kvHeads * headDim]) to row lengths[b] + i, i < pathCounts[b]; lengthsOut (may be NULL, may be lengths)
  * receives lengths + pathCounts.  The arrays of pointers are HOST arrays of `layers` entries.  weights (NULL, or a tensor
- * per layer) [batch, groups, capacity]: the weight at lengths[b] + path[b, i] moves to lengths[b] + i.  path is [batch, nodes].
+ * per layer) [batch, groups, capacity]: the weight at lengths[b] + path[b, i] moves to lengths[b] + i (0 if it lay past the
+ * capacity, where none was kept).  path is [batch, nodes].
  * A sequence whose path does not fit (an entry that is no node, a count past `nodes`, no room in the cache) is left as it
  * was, its length too. */
 int bf_hip_kv_commit(float* const* kCaches, float* const* vCaches, const float* const* kNew, const float* const* vNew, float* const* weights,

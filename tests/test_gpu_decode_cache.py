@@ -514,9 +514,9 @@ def test_accepted_rows_are_appended_to_every_layer(hip, rng, layers, dim, groups
         for b, rows in good.items():
             at = lengths[b]
             k[x][b, at:at + len(rows)], v[x][b, at:at + len(rows)] = kn[x][b, rows], vn[x][b, rows]
-            if w:      # a weight that would lie past the capacity was never kept and is not moved
-                moved = {n: w[x][b, :, at + i].copy() for n, i in enumerate(rows) if at + i < cap}
-                for n, value in moved.items():
+            if w:      # a weight that would lie past the capacity was never kept
+                moved = [w[x][b, :, at + i].copy() if at + i < cap else 0 for i in rows]
+                for n, value in enumerate(moved):
                     w[x][b, :, at + n] = value
         assert dev[0][x].toHost().tobytes() == k[x].tobytes() and dev[1][x].toHost().tobytes() == v[x].tobytes(), f"layer {x}"
         if w:
