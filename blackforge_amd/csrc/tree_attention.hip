@@ -67,7 +67,8 @@ struct TilePlan {
     float* scores;       // [batch][kvHeads][rows][scorePitch] dot products with the cached rows (NULL: not kept)
     float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
     int scorePitch, partPitch, keyBlocks;
-    float c;             // |scale| log2(e)
+    float c;             // |scale| log2(e); 1 if that is 0
+    float sign;          // that of the scale, which the queries take; 0 with c: a scale of 0 makes every score it sees 0
     unsigned magic;      // 2^32 / (heads / kvHeads), rounded up
 };
 
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     };
     unsigned seen[RT];   // bits 0..3: new rows 16 newTile + 4 g .. that this lane's row of tile t sees
     float q[RT][KS][4];
-    const float sign = p.scale < 0.0f ? -1.0f : 1.0f;
+    const float sign = plan.sign;
     const float* qBase = p.q + size_t(b) * p.nodes * p.heads * hd + size_t(kh) * share * hd;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -1060,6 +1061,8 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const size_t chunksAtMost = batch * std::max<size_t>(1, (capacity + plan.minChunk - 1) / plan.minChunk);
     plan.items = int(std::min(chunksAtMost, size_t(plan.target) + batch));
     plan.c = float(std::fabs(double(p.scale)) * 1.4426950408889634074);
+    plan.sign = plan.c == 0.0f ? 0.0f : p.scale < 0.0f ? -1.0f : 1.0f;
+    if (plan.c == 0.0f) plan.c = 1.0f;      // what a row does not see stays at -inf, which 0 would turn into NaN
     plan.magic = unsigned(((size_t(1) << 32) + share - 1) / share);
     plan.scorePitch = int((capacity + 15) / 16 * 16);
     plan.partPitch = int((headDim + 3) / 4 * 4);

@@ -275,6 +275,35 @@ def test_large_and_growing_scores(hip, rng):
     check_weights(got[3], weights, want[3], [600], [nodes], nodes, want[4], "growing scores")
 
 
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_any_scale(hip, rng, scale):
+    heads, hd, cap = 2, 64, 300
+    for nodes in (5, 40):
+        q, kn, vn, k, v = make(rng, 1, heads, heads, hd, nodes, cap, [260], [nodes])
+        visible = tree_masks(rng, 1, nodes)
+        want = reference(q, kn, vn, k, v, [260], [nodes], visible, heads, heads, heads, scale)
+        weights = np.ones((1, heads, cap), f32)
+        got = run_tree(hip, q, kn, vn, k, v, [260], [nodes], visible, heads, heads, scale, weights, heads)
+        check_tree(got, want, [nodes], 5.5, f"scale {scale}")
+        check_weights(got[3], weights, want[3], [260], [nodes], nodes, want[4], f"scale {scale}")
+
+
+def test_many_rows_to_a_key_head_with_values_that_are_not_finite(hip, rng):
+    """Sixty-four nodes (several row tiles): what a sibling holds touches its own descendants only."""
+    heads, hd, nodes, cap = 2, 64, 64, 200
+    visible = np.array([[1] + [1 | 1 << i for i in range(1, nodes)]], np.uint64)
+    q, kn, vn, k, v = make(rng, 1, heads, heads, hd, nodes, cap, [133], [nodes])
+    want = reference(q, kn, vn, k, v, [133], [nodes], visible, heads, heads, heads, 0.125)
+    bad_k, bad_v = kn.copy(), vn.copy()
+    bad_v[0, 5], bad_v[0, 37, 3], bad_k[0, 50] = np.nan, np.inf, np.nan
+    got = run_tree(hip, q, bad_k, bad_v, k, v, [133], [nodes], visible, heads, heads, 0.125)
+    clean = [i for i in range(nodes) if i not in (5, 37, 50)]
+    worst = np.abs(got[0][0, clean] - want[0][0, clean]).max()
+    assert worst <= 2 * want[4] * 5.5, worst
+    assert np.isnan(got[0][0, 5]).all() and np.isnan(got[0][0, 50]).all()
+    assert not np.isfinite(got[0][0, 37, 3]) and np.isfinite(np.delete(got[0][0, 37], 3)).all()
+
+
 def test_results_do_not_change_from_run_to_run(hip, rng):
     batch, heads, hd, nodes, cap = 2, 8, 64, 24, 5000
     lengths, counts = [5000, 3111], [24, 20]
