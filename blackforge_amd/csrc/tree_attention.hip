@@ -676,8 +676,8 @@ __global__ void __launch_bounds__(256, 2) keyWeightTilesKernel(KeyWeightParams p
         float top[4], over[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            over[r] = l[r] > 0.0f ? __builtin_amdgcn_rcpf(l[r]) : 0.0f;
-            top[r] = l[r] > 0.0f ? m[r] : INFINITY;      // a row that saw nothing gives nothing
+            over[r] = l[r] != 0.0f ? __builtin_amdgcn_rcpf(l[r]) : 0.0f;
+            top[r] = l[r] != 0.0f ? m[r] : INFINITY;      // a row that saw nothing gives nothing
         }
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
@@ -804,8 +804,8 @@ __global__ void __launch_bounds__(256, 2) keyWeightSplitKernel(KeyWeightParams p
             }
         }
         if (threadIdx.x < ROWS) {
-            sTop[buf][threadIdx.x] = l > 0.0f ? m : INFINITY;      // a row that saw nothing gives nothing
-            sOver[buf][threadIdx.x] = l > 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
+            sTop[buf][threadIdx.x] = l != 0.0f ? m : INFINITY;      // a row that saw nothing gives nothing
+            sOver[buf][threadIdx.x] = l != 0.0f ? __builtin_amdgcn_rcpf(l) : 0.0f;
         }
     };
     load(span.x);

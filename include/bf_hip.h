@@ -497,7 +497,8 @@ int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float
  * weightsOut[b, g, j] = weightsIn[b, g, j] + sum over the heads of group g and the queries i < counts[b] (NULL: newLen)
  * with j <= oldLen + i of exp(score_ij - m_i) / l_i, for j < totalLen; weights: [batch, groups, weightRows].  A row with
  * l = 0 gives nothing.  weightsIn may be NULL (zeros) or weightsOut itself.  oldLen >= totalLen - 1: no causal mask.
- * The q and k that count must be finite: past 64 queries the products are made of bf16 terms, which infinities have none. */
+ * The q and k that count must be finite: past 64 queries the products are made of bf16 terms, which infinities have none;
+ * a query whose m or l is NaN makes the weights of the keys it sees NaN. */
 int bf_hip_attention_key_weights(const float* q, const float* k, const float* m, const float* l, const int* counts, const float* weightsIn,
                                  float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t newLen, size_t totalLen,
                                  size_t kvRows, size_t headDim, float scale, size_t oldLen, size_t weightRows, bf_stream_t stream);

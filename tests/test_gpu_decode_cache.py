@@ -372,6 +372,20 @@ def test_weight_of_keys_from_the_statistics(hip, rng, case):
         assert (got[:, :, total:] == rest).all(), "weights past totalLen were written"
 
 
+@pytest.mark.parametrize("n", [20, 100])
+def test_statistics_that_are_nan_reach_the_keys_their_query_sees(hip, rng, n):
+    heads, hd, row = 2, 64, n - 7
+    q, k = (hip.DeviceTensor.fromHost(rng.standard_normal((1, n, heads * hd)).astype(f32)) for _ in range(2))
+    m = hip.DeviceTensor.fromHost(np.full((1, heads, n), 9, f32))
+    sums = np.ones((1, heads, n), f32)
+    sums[0, 1, row] = np.nan
+    l, out = hip.DeviceTensor.fromHost(sums), hip.DeviceTensor.zeros((1, heads, n))
+    hip.capi.call("bf_hip_attention_key_weights", q.ptr, k.ptr, m.ptr, l.ptr, None, None, out.ptr, 1, heads, heads, heads, n, n, n, hd, 0.125, 0, n, None)
+    got = out.toHost()
+    assert np.isfinite(got[0, 0]).all()
+    assert np.isnan(got[0, 1, :row + 1]).all() and np.isfinite(got[0, 1, row + 1:]).all()
+
+
 # ---- eviction ----------------------------------------------------------------------------------
 def kept_rows(weights, length, budget, recent):
     if length <= budget:
