@@ -80,7 +80,7 @@ __device__ __forceinline__ int bestChunk(const TreeParams& p, const TilePlan& pl
     const int lane = threadIdx.x & 63, mine = (length + 63) / 64;
     const float base = float(total) / plan.slots;            // units of 64 keys that fill the slots once
     const int least = plan.minChunk / 64;
-    const float size = fmaxf(float(least), ceilf(base * 1.5f * 18.0f / (18.0f + float(lane))));
+    const float size = fminf(fmaxf(float(least), ceilf(base * 1.5f * 18.0f / (18.0f + float(lane)))), 16777216.0f);   // 2^30 keys
     const float over = 1.0f / size;
     float chunks = 0.0f;
     for (int b = 0; b < p.batch; ++b) chunks += fmaxf(1.0f, ceilf(float(__builtin_amdgcn_readlane(mine, b)) * over - 1e-4f));
@@ -93,7 +93,7 @@ __device__ __forceinline__ int bestChunk(const TreeParams& p, const TilePlan& pl
         const int other = __shfl_xor(best, off, 64);
         if (otherCost < cost || (otherCost == cost && other > best)) { cost = otherCost; best = other; }
     }
-    return cost == INFINITY ? int(ceilf(base * 2.0f)) + 1 : best;
+    return cost == INFINITY ? int(fminf(ceilf(base * 2.0f) + 1.0f, 16777216.0f)) : best;
 }
 
 // Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for each (a
@@ -928,6 +928,7 @@ int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
     // 67 us with 128, 256, 512, 1024; one of 4096: 101, 95, 92, 158 with 256 to 2048)
     int chunk = 2048;
     while (chunk > 128 && blocks * size_t((p.newLen + chunk - 1) / chunk) < size_t(computeUnits()) * 3) chunk /= 2;
+    while (chunk < p.newLen && chunk < (1 << 30) && pairs * size_t((p.newLen + chunk - 1) / chunk) * p.totalLen > (size_t(1) << 28)) chunk *= 2;   // sums of 1 GiB
     p.queryChunk = chunk;
     p.queryChunks = std::max(1, (p.newLen + chunk - 1) / chunk);
     const size_t grid = blocks * p.queryChunks;
@@ -1020,7 +1021,7 @@ int checkHeads(const char* fn, size_t heads, size_t kvHeads, size_t groups, size
     if (groups == 0 || kvHeads % groups != 0)
         return failInvalid(fn, "groups (" + std::to_string(groups) + ") must divide kvHeads (" + std::to_string(kvHeads) + ")");
     if (headDim > 256) return failInvalid(fn, "headDim (" + std::to_string(headDim) + ") exceeds the supported limit (256)");
-    if (heads >= (size_t(1) << 16)) return failInvalid(fn, "shape too large");
+    if (heads >= (size_t(1) << 16) || heads / kvHeads > 4096) return failInvalid(fn, "shape too large");
     return BF_OK;
 }
 

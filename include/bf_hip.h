@@ -468,7 +468,8 @@ int bf_hip_counter_add(int* counter, int by, bf_stream_t stream);
  * kCache, vCache: [batch, capacity, kvHeads * headDim], of which the first lengths[b] rows of sequence b are in use (the
  * layout of hip::KVCache); lengths, counts and the like are int32 in DEVICE memory, one per sequence, so that a host may
  * launch ahead of the device; kernels hold them inside what the tensors have room for.  Query head h reads key head
- * h * kvHeads / heads (kvHeads must divide heads); headDim <= 256, at most 64 new tokens ("nodes") a sequence.
+ * h * kvHeads / heads (kvHeads must divide heads, at most 4096 to one); headDim <= 256, at most 64 new tokens ("nodes") a
+ * sequence.
  *
  * attention_tree: the new tokens are the nodes of a drafted tree; their keys and values, kNew and vNew [batch, nodes,
  * kvHeads * headDim], are not yet in the cache.  Node i of sequence b sees the cached rows j < lengths[b] and the new rows

@@ -34,6 +34,8 @@ CASES = [
     ("bf_hip_attention_tree", TREE, dict(out=None), "NULL"),
     ("bf_hip_attention_tree", TREE, dict(capacity=1 << 30), "too large"),
     ("bf_hip_attention_tree", TREE, dict(batch=1 << 16), "too large"),
+    ("bf_hip_attention_tree", TREE, dict(heads=8194, kvHeads=2), "too large"),
+    ("bf_hip_attention_tree", TREE, dict(heads=4096, kvHeads=4096, nodes=64, batch=60000), "too large"),
     ("bf_hip_attention_tree_weights", WEIGHTS, dict(groups=3), "groups"),
     ("bf_hip_attention_tree_weights", WEIGHTS, dict(groups=0), "groups"),
     ("bf_hip_attention_tree_weights", WEIGHTS, dict(weightsOut=None), "NULL"),
