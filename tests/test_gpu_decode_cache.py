@@ -653,10 +653,11 @@ def test_a_drafted_generation_with_a_bounded_cache(hip, rng):
         token = then
 
 
-def test_captured_and_replayed(hip, rng):
+@pytest.mark.parametrize("nodes", [5, 40])
+def test_captured_and_replayed(hip, rng, nodes):
     """A round of weights, verification, append and eviction recorded once and replayed, beside an eager run of the same."""
     D, call = hip.DeviceTensor, hip.capi.call
-    batch, heads, hd, nodes, cap, vocab, budget = 2, 4, 64, 5, 300, 200, 200
+    batch, heads, hd, cap, vocab, budget = 2, 4, 64, 300, 200, 200
     dim = heads * hd
 
     def state():
@@ -665,7 +666,7 @@ def test_captured_and_replayed(hip, rng):
                  vn=D.fromHost(rng.standard_normal((batch, nodes, dim)).astype(f32)), k=D.fromHost(rng.standard_normal((batch, cap, dim)).astype(f32)),
                  v=D.fromHost(rng.standard_normal((batch, cap, dim)).astype(f32)), w=D.fromHost(rng.random((batch, heads, cap)).astype(f32)),
                  out=D.zeros((batch, nodes, dim)), lengths=ints(hip, [190, 120]), logits=D.fromHost(rng.standard_normal((batch, nodes, vocab)).astype(f32)),
-                 parents=ints(hip, [[-1, 0, 1, 2, 3]] * batch), path=ints(hip, np.zeros((batch, nodes))), found=ints(hip, [0] * batch), next=D.zeros((batch,)))
+                 parents=ints(hip, [list(range(-1, nodes - 1))] * batch), path=ints(hip, np.zeros((batch, nodes))), found=ints(hip, [0] * batch), next=D.zeros((batch,)))
         logits, tokens = t["logits"].toHost(), rng.integers(0, vocab, (batch, nodes))
         for j in (1, 2):
             logits[:, j - 1][np.arange(batch), tokens[:, j]] = 30
@@ -699,6 +700,40 @@ def test_captured_and_replayed(hip, rng):
             assert (eager[name].toHostInts() == replayed[name].toHostInts()).all(), f"step {step}: {name}"
     assert eager["lengths"].toHostInts().tolist() == [200, 135]
     call("bf_hip_graph_destroy", graph)
+
+
+def test_rounds_on_alternating_streams(hip, rng):
+    """Weights (workspace from the pool), verification, append and eviction, each on the other stream than the last."""
+    call = hip.capi.call
+    batch, heads, hd, cap, nodes, vocab, budget = 2, 4, 64, 3000, 40, 900, 2000
+    dim = heads * hd
+    host = dict(q=rng.standard_normal((batch, nodes, dim)), kn=rng.standard_normal((batch, nodes, dim)), vn=rng.standard_normal((batch, nodes, dim)),
+                k=rng.standard_normal((batch, cap, dim)), v=rng.standard_normal((batch, cap, dim)), w=rng.random((batch, heads, cap)),
+                logits=rng.standard_normal((batch, nodes, vocab)), tokens=np.zeros((batch, nodes)), out=np.zeros((batch, nodes, dim)), next=np.zeros(batch))
+    host["logits"][:, :6, 0] = 30      # the model's choice is token 0 six times over
+
+    def run(streams):
+        t = {n: hip.DeviceTensor.fromHost(x.astype(f32)) for n, x in host.items()}
+        t.update(lengths=ints(hip, [2900, 1990]), path=ints(hip, np.zeros((batch, nodes))), found=ints(hip, [0] * batch),
+                 parents=ints(hip, [list(range(-1, nodes - 1))] * batch))
+        arrays = [(ctypes.c_void_p * 1)(t[n].ptr) for n in ("k", "v", "kn", "vn", "w")]
+        for step in range(4):
+            s = [streams[(step + i) % len(streams)].handle for i in range(4)]
+            call("bf_hip_attention_tree_weights", t["q"].ptr, t["kn"].ptr, t["vn"].ptr, t["k"].ptr, t["v"].ptr, t["lengths"].ptr, None, None, t["out"].ptr,
+                 None, None, t["w"].ptr, t["w"].ptr, batch, heads, heads, heads, nodes, cap, hd, 0.125, s[0])
+            call("bf_hip_tree_accept", t["logits"].ptr, t["tokens"].ptr, t["parents"].ptr, None, t["path"].ptr, t["found"].ptr, t["next"].ptr, batch, nodes,
+                 vocab, s[1])
+            call("bf_hip_kv_commit", *arrays, 1, t["path"].ptr, t["found"].ptr, t["lengths"].ptr, t["lengths"].ptr, batch, heads, heads, nodes, cap, hd, s[2])
+            call("bf_hip_kv_evict", t["k"].ptr, t["v"].ptr, t["w"].ptr, t["lengths"].ptr, t["k"].ptr, t["v"].ptr, t["w"].ptr, t["lengths"].ptr, None, batch,
+                 heads, heads, hd, cap, cap, budget, 16, s[3])
+        call("bf_hip_synchronize")
+        return {n: t[n].toHost().tobytes() for n in ("out", "k", "v", "w", "next")}, t["lengths"].toHostInts().tolist()
+
+    want = run([hip.Stream()])
+    assert want[1] == [2000, 2000]
+    two = [hip.Stream(), hip.Stream()]
+    for _ in range(3):
+        assert run(two) == want
 
 
 def test_caches_past_two_to_the_32_elements(hip, rng):
