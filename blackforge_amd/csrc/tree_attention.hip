@@ -63,6 +63,7 @@ struct TilePlan {
     int rowGroups;       // groups of RT row tiles
     float4v* partStat;   // [item][kvHeads][rows]: ref, l, largest dot product
     float* partOut;      // [item][kvHeads][rows][partPitch], relative to ref
+    float2* rowStat;     // [batch][kvHeads][rows]: ref, 1 / l over all chunks, for a launch that makes weights (NULL: not kept)
     int2* span;          // [batch]: first item and number of items of a sequence
     float* scores;       // [batch][kvHeads][rows][scorePitch] dot products with the cached rows (NULL: not kept)
     float* newScores;    // [batch][kvHeads][rows][64] and with the new ones, -infinity where not seen
@@ -180,6 +181,7 @@ __device__ __forceinline__ void finishStats(const TreeParams& p, const TilePlan&
     const int share = p.heads / p.kvHeads;
     const size_t stat = (size_t(b) * p.heads + kh * share + row % share) * p.nodes + row / share;
     const bool empty = sum == 0.0f;
+    if (plan.rowStat) plan.rowStat[(size_t(b) * p.kvHeads + kh) * p.nodes * share + row] = make_float2(ref, empty ? 0.0f : 1.0f / sum);
     if (p.m) p.m[stat] = empty ? -INFINITY : top * fabsf(p.scale);
     if (p.l) p.l[stat] = empty ? 0.0f : sum * __builtin_amdgcn_exp2f(-fmaf(top, plan.c, -ref));
 }
@@ -513,43 +515,38 @@ __device__ __forceinline__ float2 joinedSum(const TilePlan& plan, size_t at, siz
     return make_float2(most, sum);
 }
 
-// The weights of a block of 1024 cached rows, four a thread, from the kept dot products of the group's rows; the block of
-// the first ones also makes the new rows'.  The statistics are put together here once more, 64 rows at a time, rather than
-// waited for in a launch of their own (a step over 1500 rows, 12 heads: 15 -> 12 us).
+// The weights of a block of 1024 cached rows, four a thread, from the kept dot products of the group's rows, of which there
+// are four at most; the block of the first ones also makes the new rows'.  The statistics are put together here once more, a
+// row by each wavefront, rather than waited for in a launch of their own.
 __device__ __forceinline__ void weightsFromScores(const TreeParams& p, const TilePlan& plan, int index) {
-    __shared__ float2 sStat[64];
+    __shared__ float2 sStat[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int block = index % plan.keyBlocks, g = index / plan.keyBlocks % p.groups, b = index / plan.keyBlocks / p.groups;
     const int share = p.heads / p.kvHeads, rows = p.nodes * share, length = rowsInUse(p, b), count = nodesInUse(p, b), live = count * share;
     if (block != 0 && block * 1024 >= length) return;
     const int perGroup = p.kvHeads / p.groups, kh0 = g * perGroup, all = perGroup * live;
     const size_t at = (size_t(b) * p.groups + g) * p.capacity, step = size_t(p.kvHeads) * rows;
-    const int2 span = plan.span[b];
     const int j = block * 1024 + int(threadIdx.x) * 4, fresh = threadIdx.x;
-    const bool cached = plan.scores && j < length, isNew = block == 0 && fresh < count && length + fresh < p.capacity;
+    const bool cached = j < length, isNew = block == 0 && fresh < count && length + fresh < p.capacity;
+    if (wave < all) {
+        const int2 span = plan.span[b];
+        float mx;
+        const float2 st = joinedSum<64>(plan, size_t(span.x) * step + size_t(kh0 + wave / live) * rows + wave % live, step, span.y, mx);
+        if (lane == 0) sStat[wave] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
+    }
+    __syncthreads();
     float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float newSum = 0.0f;
-    for (int n0 = 0; n0 < all; n0 += 64) {
-        const int batch = min(64, all - n0);
-        for (int n = wave; n < batch; n += 4) {
-            const int kh = kh0 + (n0 + n) / live, row = (n0 + n) % live;
-            float mx;
-            const float2 st = joinedSum<64>(plan, size_t(span.x) * step + size_t(kh) * rows + row, step, span.y, mx);
-            if (lane == 0) sStat[n] = make_float2(st.x, st.y == 0.0f ? 0.0f : 1.0f / st.y);
-        }
-        __syncthreads();
 #pragma unroll 4
-        for (int n = 0; n < batch; ++n) {
-            const size_t row = (size_t(b) * p.kvHeads + kh0 + (n0 + n) / live) * rows + (n0 + n) % live;
-            const float2 st = sStat[n];
-            if (cached) {
-                const float4v x = loadf4(plan.scores + row * plan.scorePitch + j);
+    for (int n = 0; n < all; ++n) {
+        const size_t row = (size_t(b) * p.kvHeads + kh0 + n / live) * rows + n % live;
+        const float2 st = sStat[n];
+        if (cached) {
+            const float4v x = loadf4(plan.scores + row * plan.scorePitch + j);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
-            }
-            if (isNew) newSum += __builtin_amdgcn_exp2f(fmaf(plan.newScores[row * 64 + fresh], plan.c, -st.x)) * st.y;
+            for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
         }
-        __syncthreads();
+        if (isNew) newSum += __builtin_amdgcn_exp2f(fmaf(plan.newScores[row * 64 + fresh], plan.c, -st.x)) * st.y;
     }
     if (cached) {
 #pragma unroll
@@ -557,6 +554,44 @@ __device__ __forceinline__ void weightsFromScores(const TreeParams& p, const Til
             if (j + e < length) p.weightsOut[at + j + e] = (p.weightsIn ? p.weightsIn[at + j + e] : 0.0f) + sum[e];
     }
     if (isNew) p.weightsOut[at + length + fresh] = newSum;
+}
+
+// The weights of 64 cached rows from the kept dot products and the rows' statistics, or (block 0) those of the new rows, in
+// a launch of its own: sixteen lanes have four keys each, and the sixteen such groups take every sixteenth row.
+__global__ void __launch_bounds__(256) rowWeightsKernel(TreeParams p, TilePlan plan) {
+    __shared__ float4v sSum[16][17];
+    const int sub = threadIdx.x & 15, part = threadIdx.x >> 4;
+    const int block = blockIdx.x % plan.keyBlocks, g = blockIdx.x / plan.keyBlocks % p.groups, b = blockIdx.x / plan.keyBlocks / p.groups;
+    const int share = p.heads / p.kvHeads, rows = p.nodes * share, length = rowsInUse(p, b), count = nodesInUse(p, b), live = count * share;
+    const int first = block == 0 ? 0 : (block - 1) * 64, keys = block == 0 ? min(count, p.capacity - length) : min(64, length - first);
+    if (keys <= 0) return;
+    const int perGroup = p.kvHeads / p.groups;
+    const size_t pitch = block == 0 ? 64 : plan.scorePitch, row0 = (size_t(b) * p.kvHeads + size_t(g) * perGroup) * rows;
+    const float* from = (block == 0 ? plan.newScores : plan.scores) + row0 * pitch + min(first + sub * 4, int(pitch) - 4);
+    const float2* stat = plan.rowStat + row0;
+    const int over = max(1, live), khStep = 16 / over, rowStep = 16 % over;
+    int kh = part / over, row = part % over;
+    float4v sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int n = part; n < perGroup * live; n += 16) {
+        const size_t at = size_t(kh) * rows + row;
+        const float2 st = stat[at];
+        const float4v x = loadf4(from + at * pitch);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __builtin_amdgcn_exp2f(fmaf(x[e], plan.c, -st.x)) * st.y;
+        row += rowStep;
+        kh += khStep + (row >= live);
+        row -= row >= live ? live : 0;
+    }
+    sSum[part][sub] = sum;
+    __syncthreads();
+    if (int(threadIdx.x) >= keys) return;
+    const int of = threadIdx.x / 4, e = threadIdx.x % 4;
+    float all = 0.0f;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) all += sSum[n][of][e];
+    const size_t at = (size_t(b) * p.groups + g) * p.capacity + (block == 0 ? length : first) + threadIdx.x;
+    p.weightsOut[at] = block != 0 && p.weightsIn ? p.weightsIn[at] + all : all;
 }
 
 // The chunks of a row put together.  LPR lanes hold a row's columns, four each.  Few chunks a row (MANY false): every LPR
@@ -1069,16 +1104,20 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     plan.partPitch = int((headDim + 3) / 4 * 4);
     const bool join = size_t(plan.items) > batch;
     const size_t slots = size_t(plan.items) * kvHeads * rows, rowsAll = batch * kvHeads * rows;
-    plan.keyBlocks = keepScores ? std::max(1, int((capacity + 1023) / 1024)) : 1;
+    // The join's launch makes the weights too where a group has a row for each wavefront of its workgroups at most: they put the
+    // statistics together themselves (1024 rows, 12 groups of one head: 11 us against 14).  Else a launch of its own with the
+    // statistics from the join (12 nodes, one group of 12 heads: 16 us against 123; 8 groups, 8192 rows: 46 against 48).
+    const bool apart = recompute || (keepScores && kvHeads / groups * rows > 4);
+    plan.keyBlocks = !keepScores ? 1 : apart ? int((capacity + 63) / 64) + 1 : int((capacity + 1023) / 1024);
     const size_t weightBlocks = weights && capacity != 0 ? batch * groups * size_t(plan.keyBlocks) : 0;
     if (rowsAll + weightBlocks >= (size_t(1) << 31) || size_t(plan.items) * kvHeads * size_t(plan.rowGroups) >= (size_t(1) << 31))
         return failInvalid(fn, "shape too large");
-    const size_t need[] = {join || weights ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
+    const size_t need[] = {join || (weights && !apart) ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
                            keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, weights ? rowsAll * 64 * sizeof(float) : 0,
-                           recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0};
+                           recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0, apart ? rowsAll * sizeof(float2) : 0};
     hipStream_t s = asStream(stream);
-    size_t bytes = 0, offset[6];
-    for (int i = 0; i < 6; ++i) {
+    size_t bytes = 0, offset[7];
+    for (int i = 0; i < 7; ++i) {
         offset[i] = bytes;
         bytes += (need[i] + 255) / 256 * 256;
     }
@@ -1090,6 +1129,7 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     plan.span = reinterpret_cast<int2*>(part(2));
     plan.scores = reinterpret_cast<float*>(part(3));
     plan.newScores = reinterpret_cast<float*>(part(4));
+    plan.rowStat = reinterpret_cast<float2*>(part(6));
     if (float* own2 = reinterpret_cast<float*>(part(5))) {
         if (!p.m) p.m = own2;
         if (!p.l) p.l = own2 + rowsAll;
@@ -1099,8 +1139,12 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     st = launchTiles(p, plan, hdp, rt, mode, grid, s);
     if (st != BF_OK) return st;
     // the new rows' weights, and the cached rows' where their dot products were kept, ride on the launch that joins
-    st = launchJoin(p, plan, rowsAll, weightBlocks, s);
+    st = launchJoin(p, plan, rowsAll, apart ? 0 : weightBlocks, s);
     if (st != BF_OK) return st;
+    if (apart) {
+        rowWeightsKernel<<<unsigned(weightBlocks), 256, 0, s>>>(p, plan);
+        BF_LAUNCH_CHECK();
+    }
     if (recompute) {
         KeyWeightParams w{};
         w.q = p.q; w.k = p.k; w.m = p.m; w.l = p.l; w.counts = p.counts; w.lengths = p.lengths; w.weightsIn = p.weightsIn; w.weightsOut = p.weightsOut;
