@@ -157,23 +157,37 @@ __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& 
     return c;
 }
 
-// MODE 2: headDim == HDP, 16-byte aligned; 1: a multiple of 4, aligned; 0: anything
+// Columns d .. of a row.  MODE 2: headDim == HDP, 16-byte aligned; 1: a multiple of 4, aligned; 0: anything.  `sure`: the
+// caller's form is for head dims that all have these columns.  With mode 1 the columns past the row's end hold any others of
+// it, and the caller takes them out where it uses them: a select behind a load waits for it (head dim 100, 4 x 8192 rows, 8
+// heads: 80 us with the select here, 59 without; 160: 135 and 111; one element at a time the select is better, 33: 36 and 42).
 template <int MODE, int W>
-__device__ __forceinline__ void loadColumns(float (&x)[W], const float* row, int d, int hd) {
+__device__ __forceinline__ void fetchColumns(float (&x)[W], const float* row, int d, int hd, bool sure = false) {
     if constexpr (MODE == 0) {
 #pragma unroll
-        for (int j = 0; j < W; ++j) x[j] = d + j < hd ? row[d + j] : 0.0f;
+        for (int j = 0; j < W; ++j) x[j] = sure || d + j < hd ? row[d + j] : 0.0f;
     } else {
-        const bool in = MODE == 2 || d < hd;
-        const float* at = row + (in ? d : 0);
+        const float* at = row + (MODE == 2 || sure || d < hd ? d : 0);
         if constexpr (W == 4) {
             const float4v f = loadf4(at);
-            x[0] = in ? f.x : 0.0f; x[1] = in ? f.y : 0.0f; x[2] = in ? f.z : 0.0f; x[3] = in ? f.w : 0.0f;
+            x[0] = f.x; x[1] = f.y; x[2] = f.z; x[3] = f.w;
         } else {
             const float2v f = *reinterpret_cast<const float2v*>(at);
-            x[0] = in ? f.x : 0.0f; x[1] = in ? f.y : 0.0f;
+            x[0] = f.x; x[1] = f.y;
         }
     }
+}
+template <int MODE, int W>
+__device__ __forceinline__ void clearPastEnd(float (&x)[W], int d, int hd) {
+    if constexpr (MODE == 1) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) x[j] = d < hd ? x[j] : 0.0f;
+    }
+}
+template <int MODE, int W>
+__device__ __forceinline__ void loadColumns(float (&x)[W], const float* row, int d, int hd) {
+    fetchColumns<MODE>(x, row, d, hd);
+    clearPastEnd<MODE>(x, d, hd);
 }
 
 // A row's statistics from its reference, the sum about it and its largest dot product
@@ -193,11 +207,12 @@ constexpr float kRefSlack = 8.0f;
 __device__ __forceinline__ int nodeOf(const TilePlan& plan, int share, int row) { return share == 1 ? row : int(__umulhi(unsigned(row), plan.magic)); }
 
 // wavefronts per SIMD that the registers of a form allow
-constexpr int tileWaves(int hdp, int rt) { return hdp * rt <= 64 ? 3 : hdp * rt <= 256 && hdp <= 128 ? 2 : 1; }
+constexpr int tileWaves(int hdp, int rt) { return hdp * rt <= 96 ? 3 : hdp * rt <= 256 && hdp <= 128 ? 2 : 1; }
 template <int HDP, int RT, int MODE, bool SCORES>
 __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeParams p, TilePlan plan) {
     constexpr int KS = HDP / 16;                    // 16-column steps of the dot products
-    constexpr int VW = HDP >= 64 ? 4 : 2;           // value columns a lane loads at once
+    constexpr int LEAST = HDP == 256 ? 192 : HDP == 192 ? 128 : HDP == 32 ? 0 : HDP - 32;   // head dims of this form are above
+    constexpr int VW = HDP % 64 == 0 ? 4 : 2;       // value columns a lane loads at once
     constexpr int VU = HDP / (16 * VW);             // such loads
     constexpr int PITCH = HDP + 4;
     extern __shared__ float smem[];                 // [wavefront][row][PITCH]: the outputs to be joined
@@ -233,14 +248,14 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
     auto loadK = [&](const float* base, int last) {
         const float* src = reinterpret_cast<const float*>(reinterpret_cast<const char*>(base) + 4u * (__umul24(unsigned(min(i16, last)), kvDim) + 4 * g));
 #pragma unroll
-        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(k[s], src - 4 * g, 16 * s + 4 * g, hd);
+        for (int s = 0; s < KS; ++s) fetchColumns<MODE>(k[s], src - 4 * g, 16 * s + 4 * g, hd, 16 * s + 16 <= LEAST);
     };
     auto loadV = [&](const float* base, int last) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float* src = reinterpret_cast<const float*>(reinterpret_cast<const char*>(base) + 4u * __umul24(unsigned(min(4 * g + r, last)), kvDim));
 #pragma unroll
-            for (int u = 0; u < VU; ++u) loadColumns<MODE, VW>(v[u][r], src, u * 16 * VW + i16 * VW, hd);
+            for (int u = 0; u < VU; ++u) fetchColumns<MODE>(v[u][r], src, u * 16 * VW + i16 * VW, hd, (u + 1) * 16 * VW <= LEAST);   // past the end: columns that nobody reads
         }
     };
     unsigned seen[RT];   // bits 0..3: new rows 16 newTile + 4 g .. that this lane's row of tile t sees
@@ -272,6 +287,11 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
             for (int w = 0; w < VW; ++w) o[t][u][w] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
     }
     const int newLast = min(15, count - 1 - newTile * 16);
+    auto clearKeys = [&]() {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+            if (16 * s + 16 > LEAST) clearPastEnd<MODE>(k[s], 16 * s + 4 * g, hd);
+    };
     auto dotProducts = [&](int t) {
         float4v even = {0.0f, 0.0f, 0.0f, 0.0f}, odd = even;   // two chains: half the error, and none waits for the one before
 #pragma unroll
@@ -346,6 +366,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
             const float* vNext = more ? vAt + size_t(64) * kvDim : hasNew ? p.vNew + firstNew : vAt;
             const int lastNext = more ? min(15, ch.end - 1 - key - 64) : hasNew ? newLast : 0;
             float x[RT][4];
+            clearKeys();
 #pragma unroll
             for (int t = 0; t < N; ++t) {
                 const float4v dots = dotProducts(t);
@@ -396,6 +417,7 @@ __global__ void __launch_bounds__(256, tileWaves(HDP, RT)) treeTilesKernel(TreeP
                     }
             if (notFinite) atomicOr(&sOdd[newTile], notFinite);
             float x[RT][4];
+            clearKeys();
 #pragma unroll
             for (int t = 0; t < N; ++t) {
                 const float4v dots = dotProducts(t);
@@ -694,7 +716,7 @@ __global__ void __launch_bounds__(256, 2) keyWeightTilesKernel(KeyWeightParams p
     auto load = [&](int i) {
         const float* src = qb + size_t(min(i + i16, span.y - 1)) * dim;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) loadColumns<MODE, 4>(q[s], src, 16 * s + 4 * g, hd);
+        for (int s = 0; s < KS; ++s) fetchColumns<MODE>(q[s], src, 16 * s + 4 * g, hd);   // past the end they meet zeros of the keys
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = min(i + 4 * g + r, span.y - 1);
@@ -815,8 +837,8 @@ __global__ void __launch_bounds__(256, 2) keyWeightSplitKernel(KeyWeightParams p
             const int e = int(threadIdx.x) + 256 * u, row = e / (HDP / 8), col = e % (HDP / 8) * 8;
             if (CHUNKS % 256 == 0 || e < CHUNKS) {
                 const float* src = qb + size_t(min(i0 + row, span.y - 1)) * dim;
-                loadColumns<MODE, 4>(q[u][0], src, col, hd);
-                loadColumns<MODE, 4>(q[u][1], src, col + 4, hd);
+                fetchColumns<MODE>(q[u][0], src, col, hd);       // past the end they meet zeros of the keys
+                fetchColumns<MODE>(q[u][1], src, col + 4, hd);
             }
         }
         if (threadIdx.x < ROWS) {
@@ -1001,12 +1023,10 @@ int launchTilesOf(const TreeParams& p, const TilePlan& plan, unsigned grid, hipS
 }
 template <int HDP, int RT>
 int launchTilesMode(const TreeParams& p, const TilePlan& plan, int mode, unsigned grid, hipStream_t s) {
-    if constexpr (RT == 1) {   // dot products are kept for up to 16 rows only
-        if (plan.scores) {
-            if (mode == 2) return launchTilesOf<HDP, RT, 2, true>(p, plan, grid, s);
-            if (mode == 1) return launchTilesOf<HDP, RT, 1, true>(p, plan, grid, s);
-            return launchTilesOf<HDP, RT, 0, true>(p, plan, grid, s);
-        }
+    if (plan.scores) {
+        if (mode == 2) return launchTilesOf<HDP, RT, 2, true>(p, plan, grid, s);
+        if (mode == 1) return launchTilesOf<HDP, RT, 1, true>(p, plan, grid, s);
+        return launchTilesOf<HDP, RT, 0, true>(p, plan, grid, s);
     }
     if (mode == 2) return launchTilesOf<HDP, RT, 2, false>(p, plan, grid, s);
     if (mode == 1) return launchTilesOf<HDP, RT, 1, false>(p, plan, grid, s);
@@ -1026,6 +1046,7 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
     switch (hdp) {
         case 32: return launchTilesRows<32>(p, plan, rt, mode, grid, s);
         case 64: return launchTilesRows<64>(p, plan, rt, mode, grid, s);
+        case 96: return launchTilesRows<96>(p, plan, rt, mode, grid, s);
         case 128: return launchTilesRows<128>(p, plan, rt, mode, grid, s);
         case 192: return launchTilesRows<192>(p, plan, rt, mode, grid, s);
         default: return launchTilesRows<256>(p, plan, rt, mode, grid, s);
@@ -1072,10 +1093,14 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.nodes = int(nodes);
     p.capacity = int(capacity); p.hd = int(headDim);
     const size_t share = heads / kvHeads, rows = nodes * share;
-    const bool keepScores = weights && capacity != 0 && rows <= 16;
+    // The weights come from the dot products that the pass leaves in a workspace, up to 1 GiB of it (or 64 bytes a key and key
+    // head); past that they are made again from the keys (20 nodes over 4 x 8192 rows, 8 heads of 64: 50 us against 66; 64
+    // nodes 78 against 97; 512 rows to a key head 484 against 514).
+    const size_t scoreBytes = batch * kvHeads * rows * ((capacity + 15) / 16 * 16) * sizeof(float);
+    const bool keepScores = weights && capacity != 0 && (rows <= 16 || scoreBytes <= size_t(1) << 30);
     const bool recompute = weights && capacity != 0 && !keepScores;
     // Row tiles a wavefront holds: what the rows fill, up to the registers there are
-    const int hdp = paddedHeadDim(headDim);
+    const int hdp = headDim > 64 && headDim <= 96 ? 96 : paddedHeadDim(headDim);
     const int most = hdp <= 64 ? 4 : hdp <= 128 ? 2 : 1;
     const int rt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
     TilePlan plan{};

@@ -140,6 +140,11 @@ TREES = [
     (1, 2, 2, 192, 12, 200, [161], [12]),
     (2, 2, 2, 256, 40, 150, [150, 3], [40, 7]),
     (1, 4, 2, 252, 64, 90, [77], [64]),
+    (2, 2, 2, 80, 40, 500, [499, 64], [40, 33]),
+    (1, 4, 2, 96, 9, 700, [700], [9]),
+    (2, 2, 1, 81, 7, 300, [299, 17], [7, 7]),
+    (1, 2, 2, 160, 20, 330, [330], [20]),
+    (1, 12, 12, 40, 2, 1000, [1000], [2]),
     (1, 2, 2, 64, 8, 20000, [19999], [8]),
     (5, 16, 16, 128, 3, 3000, [2999, 0, 1024, 5, 2048], [3, 3, 1, 2, 3]),
     (12, 2, 2, 64, 20, 3000, [3000] * 12, [0] * 11 + [20]),                       # sequences without nodes, with long caches
@@ -288,6 +293,18 @@ def test_any_scale(hip, rng, scale):
         check_weights(got[3], weights, want[3], [260], [nodes], nodes, want[4], f"scale {scale}")
 
 
+def test_weights_of_rows_too_many_to_keep_their_products(hip, rng):
+    """4096 rows to the key head over room for 66000: their dot products would be more than 1 GiB."""
+    heads, hd, nodes, cap = 64, 4, 64, 66000
+    q, kn, vn, k, v = make(rng, 1, heads, 1, hd, nodes, cap, [300], [nodes])
+    visible = tree_masks(rng, 1, nodes)
+    want = reference(q, kn, vn, k, v, [300], [nodes], visible, heads, 1, 1, 0.5)
+    weights = np.ones((1, 1, cap), f32)
+    got = run_tree(hip, q, kn, vn, k, v, [300], [nodes], visible, heads, 1, 0.5, weights, 1)
+    check_tree(got, want, [nodes], 5.5, "rows too many to keep")
+    check_weights(got[3], weights, want[3], [300], [nodes], heads * nodes, want[4], "rows too many to keep")
+
+
 def test_many_rows_to_a_key_head_with_values_that_are_not_finite(hip, rng):
     """Sixty-four nodes (several row tiles): what a sibling holds touches its own descendants only."""
     heads, hd, nodes, cap = 2, 64, 64, 200
@@ -333,6 +350,8 @@ KEYS = [
     (1, 2, 2, 2, 64, 50, 80, 80, 80, None),        # every key visible to every query
     (1, 2, 2, 2, 64, 3, 2000, 2000, 1997, None),
     (1, 3, 3, 3, 64, 1500, 1500, 1500, 0, None),
+    (1, 2, 2, 2, 80, 120, 120, 120, 0, None),
+    (1, 2, 1, 1, 160, 50, 130, 130, 80, None),
     (2, 2, 2, 2, 64, 60, 100, 100, 10, None),      # keys 70.. that no query sees
 ]
 
