@@ -121,7 +121,8 @@ __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& 
         total = __shfl(total, 0, 64);
     }
     int units = int(min((total + plan.target - 1) / plan.target, (long long)(1 << 24)));
-    if (plan.slots > 0 && p.batch <= 64) units = bestChunk(p, plan, length0, int(total));
+    // (lengths that fill the slots with the shortest chunks at most need no choice)
+    if (plan.slots > 0 && p.batch <= 64 && float(total) > plan.slots * float(plan.minChunk / 64)) units = bestChunk(p, plan, length0, int(total));
     const int size = max(plan.minChunk, units * 64);
     Chunk c{-1, 0, 0, 0, 0, 0};
     int before = 0;
@@ -1037,7 +1038,7 @@ int launchTilesRows(const TreeParams& p, const TilePlan& plan, int rt, int mode,
     if constexpr (HDP <= 64) {
         if (rt == 4) return launchTilesMode<HDP, 4>(p, plan, mode, grid, s);
     }
-    if constexpr (HDP <= 128) {
+    if constexpr (HDP <= 192) {
         if (rt == 2) return launchTilesMode<HDP, 2>(p, plan, mode, grid, s);
     }
     return launchTilesMode<HDP, 1>(p, plan, mode, grid, s);
@@ -1099,23 +1100,31 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const size_t scoreBytes = batch * kvHeads * rows * ((capacity + 15) / 16 * 16) * sizeof(float);
     const bool keepScores = weights && capacity != 0 && (rows <= 16 || scoreBytes <= size_t(1) << 30);
     const bool recompute = weights && capacity != 0 && !keepScores;
-    // Row tiles a wavefront holds: what the rows fill, up to the registers there are
+    // Row tiles a wavefront holds: what the rows fill, up to the registers there are (two tiles of 192 columns halve the reads, 142
+    // -> 90 us for 17 nodes over 4 x 8192 rows, 8 heads; of 256 they spill, 195 -> 324).  With less to do, two at most, and one
+    // where the tiles of all sequences are half the compute units at most: more workgroups, and each starts and ends sooner.  The
+    // measure is keys (by the capacity) x row tiles x columns, 0.75 and 2 times 2^18 of them a compute unit.  53 nodes over 700 rows, 8
+    // heads of 64: 11, 14, 19 us with one, two, four; over 30000 rows 49, 51, 54; over 10 x 2000 55, 48, 51; 64 nodes over 32
+    // ragged sequences, 12 heads: 188, 155, 147; heads of 128, 24 nodes over 3 x 8000 rows: 52, 56, 53 nodes 87, 76.
     const int hdp = headDim > 64 && headDim <= 96 ? 96 : paddedHeadDim(headDim);
-    const int most = hdp <= 64 ? 4 : hdp <= 128 ? 2 : 1;
+    const size_t device = size_t(computeUnits()), tiles = batch * kvHeads * ((rows + 15) / 16);
+    const double work = double(tiles) * double(capacity) * hdp / double(device << 18);
+    const int most = work <= 0.75 && tiles * 2 <= device ? 1 : hdp <= 64 && work > 2.0 ? 4 : hdp <= 192 ? 2 : 1;
     const int rt = std::min(most, rows <= 16 ? 1 : rows <= 32 ? 2 : 4);
     TilePlan plan{};
     plan.rowGroups = int((rows + 16 * rt - 1) / (16 * rt));
     plan.minChunk = 128;
-    // One row tile: the pass is a stream, and eight workgroups a compute unit in even shares keep it full (16 ragged sequences of
-    // up to 16000 rows: 400 us with four, 376 with eight).  More: chunk sizes by the rounds they make (bestChunk), with the
-    // workgroups whose registers a compute unit holds; even shares of four a compute unit measured 337 us where that gives 327
-    // (26 nodes over 120011 rows) and 160 where it gives 151 (50000 rows), and the other way round 112 and 114 us (16 nodes of
-    // four heads each over 8 ragged sequences).
-    const size_t device = size_t(computeUnits()), pairs = kvHeads * size_t(plan.rowGroups);
-    if (rt == 1) {
+    // Chunk sizes by the rounds they make (bestChunk): with several row tiles on the workgroups whose registers a compute unit
+    // holds (even shares of four a compute unit measured 337 us where that gives 327, 26 nodes over 120011 rows, and 160 where it
+    // gives 151, 50000 rows), with one on the compute units, since longer chunks cost less than they lose in loads under way (one
+    // node over 100000 rows, 2 heads of 64: 26 us, and 45 with even shares of eight a compute unit; 4 x 8192 rows, 8 heads of
+    // 192: 84 and 109).  Many sequences: a chunk more or less of each matters too much, and the even shares of eight balance
+    // them better (16 ragged sequences of up to 16000 rows, 16 heads of 128: 376 us, by rounds 387).
+    const size_t pairs = kvHeads * size_t(plan.rowGroups);
+    if (rt == 1 && batch * pairs * 2 > device) {
         plan.target = int(std::max<size_t>(1, device * 8 / pairs));
     } else {
-        plan.slots = float(device * (hdp * rt <= 128 ? 3 : 2)) / float(pairs);
+        plan.slots = float(device * (rt == 1 ? 1 : hdp * rt <= 128 ? 3 : hdp <= 128 ? 2 : 1)) / float(pairs);
         plan.target = int(std::max<size_t>(1, size_t(3.0f * plan.slots + 0.5f))) + int(batch);
     }
     // Even shares are at most target + batch chunks, and so are those of bestChunk, whose own count may miss one a sequence

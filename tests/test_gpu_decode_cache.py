@@ -151,6 +151,23 @@ TREES = [
     (9, 3, 3, 64, 40, 2100, [2100, 64, 0, 2099, 700, 1, 1337, 63, 65], [40, 33, 40, 1, 17, 40, 0, 40, 16]),
     (66, 4, 2, 128, 12, 400, [(61 * i) % 401 for i in range(66)], [(5 * i) % 13 for i in range(66)]),
     (70, 2, 2, 64, 2, 50, [(7 * i) % 51 for i in range(70)], [i % 3 for i in range(70)]),
+    # enough rows, or rows and room, for the forms that hold two and four tiles of rows
+    (1, 33, 1, 64, 63, 16400, [8137], [63]),
+    (1, 33, 1, 64, 63, 16400, [130], [40]),
+    (2, 40, 2, 32, 50, 18000, [300, 9000], [50, 41]),
+    (2, 34, 2, 60, 63, 8400, [77, 4900], [9, 63]),
+    (1, 33, 1, 33, 63, 16400, [1021], [63]),
+    (1, 33, 1, 64, 63, 300, [299], [63]),
+    (1, 33, 1, 20, 63, 300, [237], [61]),
+    (1, 33, 1, 96, 63, 300, [300], [62]),
+    (1, 33, 1, 80, 63, 700, [650], [63]),
+    (1, 33, 1, 81, 63, 100, [37], [63]),
+    (2, 66, 2, 128, 33, 700, [700, 0], [33, 30]),
+    (1, 33, 1, 100, 63, 300, [170], [63]),
+    (2, 33, 1, 192, 63, 500, [500, 1], [63, 17]),
+    (1, 33, 1, 160, 63, 300, [300], [63]),
+    (1, 33, 1, 189, 63, 200, [100], [63]),
+    (1, 33, 1, 256, 63, 200, [200], [63]),
 ]
 
 
@@ -305,20 +322,22 @@ def test_weights_of_rows_too_many_to_keep_their_products(hip, rng):
     check_weights(got[3], weights, want[3], [300], [nodes], heads * nodes, want[4], "rows too many to keep")
 
 
-def test_many_rows_to_a_key_head_with_values_that_are_not_finite(hip, rng):
-    """Sixty-four nodes (several row tiles): what a sibling holds touches its own descendants only."""
-    heads, hd, nodes, cap = 2, 64, 64, 200
+@pytest.mark.parametrize("heads,cap", [(1, 200), (33, 200), (33, 16600)])
+def test_many_rows_to_a_key_head_with_values_that_are_not_finite(hip, rng, heads, cap):
+    """Sixty-four nodes, one to four tiles of rows at a time: what a sibling holds touches its own descendants only."""
+    hd, nodes = 64, 64
     visible = np.array([[1] + [1 | 1 << i for i in range(1, nodes)]], np.uint64)
-    q, kn, vn, k, v = make(rng, 1, heads, heads, hd, nodes, cap, [133], [nodes])
-    want = reference(q, kn, vn, k, v, [133], [nodes], visible, heads, heads, heads, 0.125)
+    q, kn, vn, k, v = make(rng, 1, heads, 1, hd, nodes, cap, [133], [nodes])
+    want = reference(q, kn, vn, k, v, [133], [nodes], visible, heads, 1, 1, 0.125)
     bad_k, bad_v = kn.copy(), vn.copy()
     bad_v[0, 5], bad_v[0, 37, 3], bad_k[0, 50] = np.nan, np.inf, np.nan
-    got = run_tree(hip, q, bad_k, bad_v, k, v, [133], [nodes], visible, heads, heads, 0.125)
+    got = run_tree(hip, q, bad_k, bad_v, k, v, [133], [nodes], visible, heads, 1, 0.125)
     clean = [i for i in range(nodes) if i not in (5, 37, 50)]
     worst = np.abs(got[0][0, clean] - want[0][0, clean]).max()
     assert worst <= 2 * want[4] * 5.5, worst
     assert np.isnan(got[0][0, 5]).all() and np.isnan(got[0][0, 50]).all()
-    assert not np.isfinite(got[0][0, 37, 3]) and np.isfinite(np.delete(got[0][0, 37], 3)).all()
+    infinite = got[0][0, 37].reshape(heads, hd)
+    assert not np.isfinite(infinite[:, 3]).any() and np.isfinite(np.delete(infinite, 3, 1)).all()
 
 
 def test_results_do_not_change_from_run_to_run(hip, rng):
