@@ -52,8 +52,8 @@ __device__ __forceinline__ unsigned long long newRowsSeen(const TreeParams& p, i
 // tile normally needs no maximum across lanes and no rescaling.  d = c dot - ref in one fused operation, c = scale log2(e):
 // the error of d is relative to d, not to the score.  The true maximum is kept beside it for the statistics.
 //
-// Measured: 26 nodes, 16 heads of 128, 120011 rows 320 us = 6.1 TB/s with the join (HBM); 32 ragged sequences of up to 4032 rows,
-// 12 heads of 64, 64 nodes 146 us (427 MB, 10.3 GFLOP: the matrix instruction, 62 % busy, and the start and end of a
+// Measured: 26 nodes, 16 heads of 128, 120011 rows 322 us = 6.1 TB/s with the join (HBM); 32 ragged sequences of up to 4032 rows,
+// 12 heads of 64, 64 nodes 147 us (427 MB, 10.3 GFLOP: the matrix instruction, 62 % busy, and the start and end of a
 // workgroup, 15 us by themselves); one node over 701 rows 10 us (two dependent launches).
 struct TilePlan {
     int target;          // chunks per (key head, group of row tiles) that the launch wants in total over the sequences
