@@ -488,7 +488,8 @@ int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, 
  * divide kvHeads.  weights: [batch, groups, capacity].  For j < lengths[b] weightsOut[b, g, j] = weightsIn[b, g, j] + the
  * weight received; the new rows' weights follow at j = lengths[b] + node (where the row will be once it is appended) as far
  * as the capacity goes, without weightsIn; entries past them stay as they were.  weightsIn may be NULL (zeros) or be
- * weightsOut itself. */
+ * weightsOut itself.  Takes a workspace of 4 bytes for every row of the cache, node and query head from the pool where that
+ * is at most 1 GiB, or nodes * heads / kvHeads at most 16; else the products are made a second time. */
 int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
                                   const int* counts, const uint64_t* visible, float* out, float* m, float* l, const float* weightsIn,
                                   float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t nodes, size_t capacity,
