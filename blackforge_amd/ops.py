@@ -667,6 +667,7 @@ def kvCommit(kCaches, vCaches, kNews, vNews, accepted: AcceptedPath, lengths, we
         groups = weights[0].shape[1]
         for t in weights:
             _require(t.shape == (batch, groups, capacity), "kvCommit: weights must be [batch, groups, capacity]")
+        _require(groups > 0 and dim % groups == 0, f"kvCommit: {groups} groups do not divide rows of {dim}")
     _require(accepted.path.shape == (batch, nodes) and accepted.counts.shape == (batch,) and lengths.shape == (batch,),
              "kvCommit: one path, count and length per sequence")
     _call("bf_hip_kv_commit", _ptr_array(kCaches), _ptr_array(vCaches), _ptr_array(kNews), _ptr_array(vNews),
