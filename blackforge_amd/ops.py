@@ -567,6 +567,11 @@ def _pointer(t: Optional[DeviceTensor]):
     return t.ptr if t is not None else None
 
 
+def _ints(t: DeviceTensor, shape) -> bool:
+    """True for 32-bit device integers of this shape, as the kernels read them."""
+    return t.shape == tuple(shape) and t.itemsize == 4
+
+
 def _check_tree(name, q, kNew, vNew, kCache, vCache, lengths, numHeads, kvHeads, counts, visible):
     _require(q.rank() == 3 and kNew.rank() == 3 and kCache.rank() == 3, f"{name}: expected [batch, rows, dim] tensors")
     batch, nodes, dim = q.shape
@@ -574,7 +579,7 @@ def _check_tree(name, q, kNew, vNew, kCache, vCache, lengths, numHeads, kvHeads,
     headDim = dim // numHeads
     _require(kNew.shape == (batch, nodes, kvHeads * headDim) and vNew.shape == kNew.shape, f"{name}: incompatible new keys and values")
     _require(kCache.shape == (batch, kCache.shape[1], kvHeads * headDim) and vCache.shape == kCache.shape, f"{name}: incompatible caches")
-    _require(lengths.shape == (batch,) and (counts is None or counts.shape == (batch,)), f"{name}: one length and one count per sequence")
+    _require(_ints(lengths, (batch,)) and (counts is None or _ints(counts, (batch,))), f"{name}: one 32-bit length and count per sequence")
     _require(visible is None or (visible.shape == (batch, nodes) and visible.itemsize == 8), f"{name}: visible must be 64-bit [batch, nodes]")
     return batch, nodes, headDim
 
@@ -614,6 +619,7 @@ def attentionKeyWeights(q, k, m, l, numHeads: int, scale: float, oldLen: int, gr
     batch, newLen, dim = q.shape
     _require(numHeads > 0 and dim % numHeads == 0 and k.shape[2] == kvHeads * (dim // numHeads), "attentionKeyWeights: incompatible heads")
     _require(m.shape == (batch, numHeads, newLen) and l.shape == m.shape, "attentionKeyWeights: statistics must be [batch, heads, newLen]")
+    _require(counts is None or _ints(counts, (batch,)), "attentionKeyWeights: one 32-bit count per sequence")
     total = k.shape[1]
     out = weights if weights is not None else DeviceTensor((batch, groups, total))
     _require(out.rank() == 3 and out.shape[:2] == (batch, groups) and out.shape[2] >= total, "attentionKeyWeights: weights must be [batch, groups, rows]")
@@ -627,8 +633,8 @@ def kvEvict(kCache, vCache, weights, lengths, kvHeads: int, budget: int, recent:
     _require(kCache.rank() == 3 and vCache.shape == kCache.shape, "kvEvict: expected caches [batch, capacity, dim]")
     batch, capacity, dim = kCache.shape
     _require(kvHeads > 0 and dim % kvHeads == 0, "kvEvict: kvHeads must divide dim")
-    _require(weights.rank() == 3 and weights.shape[0] == batch and weights.shape[2] == capacity and lengths.shape == (batch,),
-             "kvEvict: weights must be [batch, groups, capacity], lengths [batch]")
+    _require(weights.rank() == 3 and weights.shape[0] == batch and weights.shape[2] == capacity and _ints(lengths, (batch,)),
+             "kvEvict: weights must be [batch, groups, capacity], lengths 32-bit [batch]")
     _call("bf_hip_kv_evict", kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, None, batch, kvHeads,
           weights.shape[1], dim // kvHeads, capacity, capacity, budget, recent, None)
 
@@ -642,9 +648,10 @@ class AcceptedPath:
 
 def treeAccept(logits, tokens, parents, counts=None) -> AcceptedPath:
     """The path of a drafted tree that greedy choices confirm, and the token after it (bf_hip_tree_accept)."""
-    _require(logits.rank() == 3 and tokens.shape == logits.shape[:2] and parents.shape == tokens.shape,
-             "treeAccept: expected logits [batch, nodes, vocab], tokens and parents [batch, nodes]")
+    _require(logits.rank() == 3 and tokens.shape == logits.shape[:2] and _ints(parents, tokens.shape),
+             "treeAccept: expected logits [batch, nodes, vocab], tokens and 32-bit parents [batch, nodes]")
     batch, nodes, vocab = logits.shape
+    _require(counts is None or _ints(counts, (batch,)), "treeAccept: one 32-bit count per sequence")
     res = AcceptedPath(DeviceTensor((batch, nodes)), DeviceTensor((batch,)), DeviceTensor.zeros((batch,)))
     _call("bf_hip_tree_accept", logits.ptr, tokens.ptr, parents.ptr, _pointer(counts), res.path.ptr, res.counts.ptr, res.next.ptr, batch, nodes, vocab,
           None)
@@ -668,8 +675,8 @@ def kvCommit(kCaches, vCaches, kNews, vNews, accepted: AcceptedPath, lengths, we
         for t in weights:
             _require(t.shape == (batch, groups, capacity), "kvCommit: weights must be [batch, groups, capacity]")
         _require(groups > 0 and dim % groups == 0, f"kvCommit: {groups} groups do not divide rows of {dim}")
-    _require(accepted.path.shape == (batch, nodes) and accepted.counts.shape == (batch,) and lengths.shape == (batch,),
-             "kvCommit: one path, count and length per sequence")
+    _require(_ints(accepted.path, (batch, nodes)) and _ints(accepted.counts, (batch,)) and _ints(lengths, (batch,)),
+             "kvCommit: one path, count and length (32-bit) per sequence")
     _call("bf_hip_kv_commit", _ptr_array(kCaches), _ptr_array(vCaches), _ptr_array(kNews), _ptr_array(vNews),
           _ptr_array(weights) if weights is not None else None, layers, accepted.path.ptr, accepted.counts.ptr, lengths.ptr, lengths.ptr, batch, groups,
           groups, nodes, capacity, dim // groups, None)

@@ -40,3 +40,43 @@ def test_commit_refuses_groups_that_do_not_divide_the_rows(calls):
     assert calls == []
     ops.kvCommit(caches, caches, new, new, accepted(2, 4), tensor(2), [tensor(2, 4, 30)])
     assert [name for name, _ in calls] == ["bf_hip_kv_commit"]
+
+
+@pytest.mark.parametrize("counts", [tensor(2), tensor(4), tensor(3, 1), tensor(3, itemsize=8), tensor(3, itemsize=2)], ids=lambda t: f"{t.shape}x{t.itemsize}")
+def test_counts_that_do_not_fit_are_refused(calls, counts):
+    """The kernels read one 32-bit count a sequence: a shorter array would be read past its end."""
+    from blackforge_amd import ops
+    q, m = tensor(3, 5, 64), tensor(3, 2, 5)
+    with pytest.raises(ValueError, match="count"):
+        ops.attentionKeyWeights(q, q, m, m, 2, 0.125, 0, 2, tensor(3, 2, 9), counts)
+    with pytest.raises(ValueError, match="count"):
+        ops.treeAccept(tensor(3, 5, 99), tensor(3, 5), tensor(3, 5), counts)
+    with pytest.raises(ValueError, match="count"):
+        ops.attentionTree(q, q, q, tensor(3, 9, 64), tensor(3, 9, 64), tensor(3), 2, 0.125, counts)
+    with pytest.raises(ValueError, match="count"):
+        ops.attentionTreeWeights(q, q, q, tensor(3, 9, 64), tensor(3, 9, 64), tensor(3), 2, 0.125, tensor(3, 2, 9), counts)
+    assert calls == []
+
+
+def test_integers_of_another_width_are_refused(calls):
+    """Lengths, parents and paths are 32-bit integers on the device: 64-bit ones would be read as pairs, 16-bit ones past their end."""
+    from blackforge_amd import ops
+    q, cache, weights = tensor(3, 5, 64), tensor(3, 9, 64), tensor(3, 2, 9)
+    for itemsize in (2, 8):
+        odd = tensor(3, itemsize=itemsize)
+        with pytest.raises(ValueError, match="length"):
+            ops.attentionTree(q, q, q, cache, cache, odd, 2, 0.125)
+        with pytest.raises(ValueError, match="length"):
+            ops.attentionTreeWeights(q, q, q, cache, cache, odd, 2, 0.125, weights)
+        with pytest.raises(ValueError, match="length"):
+            ops.kvEvict(cache, cache, weights, odd, 2, 4, 1)
+        with pytest.raises(ValueError, match="length"):
+            ops.kvCommit([cache], [cache], [q], [q], accepted(3, 5), odd)
+        with pytest.raises(ValueError, match="parents"):
+            ops.treeAccept(tensor(3, 5, 99), tensor(3, 5), tensor(3, 5, itemsize=itemsize))
+        for path in (ops.AcceptedPath(tensor(3, 5, itemsize=itemsize), tensor(3), tensor(3)), ops.AcceptedPath(tensor(3, 5), odd, tensor(3))):
+            with pytest.raises(ValueError, match="path"):
+                ops.kvCommit([cache], [cache], [q], [q], path, tensor(3))
+    with pytest.raises(ValueError, match="visible"):
+        ops.attentionTree(q, q, q, cache, cache, tensor(3), 2, 0.125, None, tensor(3, 5))
+    assert calls == []
