@@ -93,6 +93,8 @@ class DeviceTensor:
         return t
 
     def toHostInts(self) -> np.ndarray:
+        if self.itemsize not in (4, 8):
+            raise ValueError(f"toHostInts: elements of {self.itemsize} bytes are no integers, use toHost")
         out = np.empty(self.shape, np.int32 if self.itemsize == 4 else np.uint64)
         capi.call("bf_hip_memcpy_d2h", out.ctypes.data_as(ctypes.c_void_p), self.ptr, self._bytes)
         return out
@@ -104,6 +106,8 @@ class DeviceTensor:
         return t
 
     def toHost(self) -> np.ndarray:
+        if self.itemsize not in (2, 4):
+            raise ValueError(f"toHost: elements of {self.itemsize} bytes are no floats, use toHostInts")
         dtype = np.float32 if self.itemsize == 4 else np.uint16
         out = np.empty(self.shape, dtype)
         capi.call("bf_hip_memcpy_d2h", out.ctypes.data_as(ctypes.c_void_p), self.ptr, self._bytes)

@@ -80,3 +80,26 @@ def test_integers_of_another_width_are_refused(calls):
     with pytest.raises(ValueError, match="visible"):
         ops.attentionTree(q, q, q, cache, cache, tensor(3), 2, 0.125, None, tensor(3, 5))
     assert calls == []
+
+
+def test_masks_come_back_as_integers_only(monkeypatch):
+    """A tensor of 64-bit masks has no floats to give: copied into a float buffer it would run past that buffer's end."""
+    import numpy as np
+    from blackforge_amd import capi
+    copied = []
+    monkeypatch.setattr(capi, "call", lambda name, *args: copied.append(args[2]))
+    masks, ints, halves = tensor(3, 5, itemsize=8), tensor(3, 5), tensor(3, 5, itemsize=2)
+    for t in (masks, ints, halves):
+        t._bytes = 15 * t.itemsize
+    try:
+        with pytest.raises(ValueError, match="toHostInts"):
+            masks.toHost()
+        with pytest.raises(ValueError, match="toHost"):
+            halves.toHostInts()
+        assert copied == []
+        for got in (masks.toHostInts(), ints.toHostInts(), ints.toHost(), halves.toHost()):
+            assert got.nbytes == copied.pop()
+        assert (masks.toHostInts().dtype, ints.toHostInts().dtype) == (np.uint64, np.int32)
+    finally:
+        for t in (masks, ints, halves):
+            t._bytes = 0
