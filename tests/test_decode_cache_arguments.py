@@ -97,8 +97,8 @@ def test_masks_come_back_as_integers_only(monkeypatch):
         with pytest.raises(ValueError, match="toHost"):
             halves.toHostInts()
         assert copied == []
-        for got in (masks.toHostInts(), ints.toHostInts(), ints.toHost(), halves.toHost()):
-            assert got.nbytes == copied.pop()
+        for read in (masks.toHostInts, ints.toHostInts, ints.toHost, halves.toHost):
+            assert read().nbytes == copied.pop()
         assert (masks.toHostInts().dtype, ints.toHostInts().dtype) == (np.uint64, np.int32)
     finally:
         for t in (masks, ints, halves):
