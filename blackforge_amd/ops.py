@@ -629,14 +629,25 @@ def attentionKeyWeights(q, k, m, l, numHeads: int, scale: float, oldLen: int, gr
 
 
 def kvEvict(kCache, vCache, weights, lengths, kvHeads: int, budget: int, recent: int) -> None:
-    """The caches, the weights and the lengths cut down in place to at most `budget` rows (bf_hip_kv_evict)."""
-    _require(kCache.rank() == 3 and vCache.shape == kCache.shape, "kvEvict: expected caches [batch, capacity, dim]")
-    batch, capacity, dim = kCache.shape
-    _require(kvHeads > 0 and dim % kvHeads == 0, "kvEvict: kvHeads must divide dim")
-    _require(weights.rank() == 3 and weights.shape[0] == batch and weights.shape[2] == capacity and _ints(lengths, (batch,)),
-             "kvEvict: weights must be [batch, groups, capacity], lengths 32-bit [batch]")
-    _call("bf_hip_kv_evict", kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, kCache.ptr, vCache.ptr, weights.ptr, lengths.ptr, None, batch, kvHeads,
-          weights.shape[1], dim // kvHeads, capacity, capacity, budget, recent, None)
+    """The caches and weights of every layer (lists of tensors, or one layer's tensors) cut down in place to at most `budget`
+    rows a sequence, and last the lengths, which the layers share (bf_hip_kv_evict).  All are checked before the first is cut."""
+    if isinstance(kCache, DeviceTensor):
+        kCache, vCache, weights = [kCache], [vCache], [weights]
+    layers = len(kCache)
+    _require(layers > 0 and len(vCache) == layers and len(weights) == layers, "kvEvict: one tensor per layer")
+    _require(len({id(t) for t in kCache}) == layers, "kvEvict: a layer can be cut once only")
+    _require(kvHeads > 0 and 0 <= recent <= budget, f"kvEvict: {recent} recent rows of a budget of {budget} for {kvHeads} heads")
+    for k, v, w in zip(kCache, vCache, weights):
+        _require(k.rank() == 3 and v.shape == k.shape, "kvEvict: expected caches [batch, capacity, dim]")
+        batch, capacity, dim = k.shape
+        _require(dim % kvHeads == 0 and budget <= capacity, "kvEvict: kvHeads must divide dim, the budget must fit the capacity")
+        _require(w.rank() == 3 and w.shape[0] == batch and w.shape[2] == capacity and w.shape[1] > 0 and kvHeads % w.shape[1] == 0,
+                 "kvEvict: weights must be [batch, groups, capacity], their groups a divisor of kvHeads")
+        _require(_ints(lengths, (batch,)), "kvEvict: lengths must be 32-bit [batch]")
+    for i, (k, v, w) in enumerate(zip(kCache, vCache, weights)):
+        batch, capacity, dim = k.shape
+        _call("bf_hip_kv_evict", k.ptr, v.ptr, w.ptr, lengths.ptr, k.ptr, v.ptr, w.ptr, lengths.ptr if i + 1 == layers else None, None, batch, kvHeads,
+              w.shape[1], dim // kvHeads, capacity, capacity, budget, recent, None)
 
 
 @dataclass

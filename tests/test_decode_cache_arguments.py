@@ -103,3 +103,59 @@ def test_masks_come_back_as_integers_only(monkeypatch):
     finally:
         for t in (masks, ints, halves):
             t._bytes = 0
+
+
+def evict_layers(n=3):
+    return [tensor(2, 30, 64) for _ in range(n)], [tensor(2, 30, 64) for _ in range(n)], [tensor(2, 4, 30) for _ in range(n)]
+
+
+def test_eviction_cuts_the_lengths_with_the_last_layer(calls):
+    """The layers share their lengths: cut with the first, they would tell the others that nothing is left to evict."""
+    from blackforge_amd import ops
+    k, v, w = evict_layers()
+    lengths = tensor(2)
+    lengths.ptr = ctypes.c_void_p(2 * A)
+    ops.kvEvict(k, v, w, lengths, 8, 12, 3)
+    assert [name for name, _ in calls] == ["bf_hip_kv_evict"] * 3
+    assert [args[7] for _, args in calls] == [None, None, lengths.ptr]
+    calls.clear()
+    ops.kvEvict(k[0], v[0], w[0], lengths, 8, 12, 3)     # one layer needs no list
+    assert [args[7] for _, args in calls] == [lengths.ptr]
+
+
+@pytest.mark.parametrize("change", ["values", "capacity", "weights", "groups", "no groups", "sequences", "rank"])
+def test_eviction_refuses_before_it_cuts_any_layer(calls, change):
+    """The third layer does not fit: the first two stay whole, since the lengths would not be cut with them."""
+    from blackforge_amd import ops
+    k, v, w = evict_layers()
+    if change == "values":
+        v[2] = tensor(2, 29, 64)
+    if change == "capacity":
+        k[2], v[2], w[2] = tensor(2, 11, 64), tensor(2, 11, 64), tensor(2, 4, 11)
+    if change == "weights":
+        w[2] = tensor(2, 4, 29)
+    if change == "groups":
+        w[2] = tensor(2, 3, 30)
+    if change == "no groups":
+        w[2] = tensor(2, 0, 30)
+    if change == "sequences":
+        k[2], v[2], w[2] = tensor(3, 30, 64), tensor(3, 30, 64), tensor(3, 4, 30)
+    if change == "rank":
+        k[2] = v[2] = tensor(60, 64)
+    with pytest.raises(ValueError, match="kvEvict"):
+        ops.kvEvict(k, v, w, tensor(2), 8, 12, 3)
+    assert calls == []
+
+
+def test_eviction_refuses_budgets_and_lists_that_do_not_fit(calls):
+    from blackforge_amd import ops
+    k, v, w = evict_layers()
+    for budget, recent in ((31, 3), (12, 13), (-1, -1), (12, -1)):
+        with pytest.raises(ValueError, match="kvEvict"):
+            ops.kvEvict(k, v, w, tensor(2), 8, budget, recent)
+    for lists in ((k, v[:2], w), (k, v, w[:1]), ([], [], []), ([k[0], k[1], k[0]], v, w)):
+        with pytest.raises(ValueError, match="kvEvict"):
+            ops.kvEvict(*lists, tensor(2), 8, 12, 3)
+    with pytest.raises(ValueError, match="kvEvict"):
+        ops.kvEvict(k, v, w, tensor(2), 7, 12, 3)
+    assert calls == []
