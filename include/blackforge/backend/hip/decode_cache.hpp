@@ -109,12 +109,20 @@ inline void attentionKeyWeights(const DeviceTensor& q, const DeviceTensor& k, co
                                        weights.dim(2), nullptr));
 }
 
-// Every layer's cache cut down in place to `budget` rows a sequence, the most recent and the heaviest, and the lengths with them.
+// Every layer's cache cut down in place to `budget` rows a sequence, the most recent and the heaviest, and the lengths with
+// them.  The lengths are cut with the last layer, so all are checked before the first: cut in part, the caches and their
+// lengths would no longer agree.
 inline void evictKeyValues(std::vector<DecodeLayer>& layers, DeviceArray<int>& lengths, std::size_t kvHeads, std::size_t budget, std::size_t recent) {
+    require(kvHeads != 0 && recent <= budget, "evictKeyValues: more recent rows than the budget holds, or no heads");
+    for (const DecodeLayer& x : layers) {
+        require(x.k.rank() == 3 && x.v.shape() == x.k.shape() && x.weights.rank() == 3 && x.weights.dim(0) == x.batch() &&
+                    x.weights.dim(2) == x.capacity() && lengths.size() == x.batch(),
+                "evictKeyValues: every layer needs weights [batch, groups, capacity], every sequence a length");
+        require(x.k.dim(2) % kvHeads == 0 && x.weights.dim(1) != 0 && kvHeads % x.weights.dim(1) == 0, "evictKeyValues: incompatible heads and groups");
+        require(budget <= x.capacity(), "evictKeyValues: the budget does not fit the capacity");
+    }
     for (std::size_t i = 0; i < layers.size(); ++i) {
         DecodeLayer& x = layers[i];
-        require(x.weights.rank() == 3 && x.k.rank() == 3 && x.weights.dim(2) == x.capacity() && lengths.size() == x.batch() && kvHeads != 0 &&
-                    x.k.dim(2) % kvHeads == 0, "evictKeyValues: every layer needs weights [batch, groups, capacity], every sequence a length");
         check(bf_hip_kv_evict(x.k.data(), x.v.data(), x.weights.data(), lengths.data(), x.k.data(), x.v.data(), x.weights.data(),
                               i + 1 == layers.size() ? lengths.data() : nullptr, nullptr, x.batch(), kvHeads, x.weights.dim(1), x.k.dim(2) / kvHeads,
                               x.capacity(), x.capacity(), budget, recent, nullptr));

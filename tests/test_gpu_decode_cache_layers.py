@@ -1,4 +1,6 @@
 """GPU tests of the cache operators over several layers that share their sequences' lengths, and at sizes with nothing in them."""
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -28,3 +30,11 @@ def test_eviction_of_layers_that_share_their_lengths(hip, rng):
                 ek[b, :len(rows), at], ev[b, :len(rows), at], ew[b, g, :len(rows)] = k[x][b, rows, at], v[x][b, rows, at], w[x][b, g, rows]
         for got, want, what in ((dk, ek, "keys"), (dv, ev, "values"), (dw, ew, "weights")):
             assert got[x].toHost().tobytes() == want.tobytes(), f"{what} of layer {x}"
+
+
+def test_the_cpp_layer_cuts_all_layers_or_none(hip):
+    """tests/cpp/decode_cache_layers_test.cpp: a layer that does not fit is refused before any other is cut."""
+    exe = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "blackforge_amd", "host", "bin", "decode_cache_layers_test")
+    assert os.path.exists(exe), "blackforge_amd/host has not been built"
+    proc = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert proc.returncode == 0, proc.stdout + proc.stderr
