@@ -370,11 +370,13 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
     BF_REQUIRE(budget <= outCapacity, "the budget does not fit the result's capacity");
     BF_REQUIRE(batch < (size_t(1) << 16) && groups < (size_t(1) << 16) && kvHeads * headDim < (size_t(1) << 24) && capacity < (size_t(1) << 30) &&
                    outCapacity < (size_t(1) << 30), "shape too large");
-    if (batch == 0 || capacity == 0 || headDim == 0) return BF_OK;
-    BF_REQUIRE(lengths && kCache && vCache && weights && ((kOut && vOut && weightsOut) || budget == 0), "NULL pointer");
+    if (batch == 0 || headDim == 0) return BF_OK;
+    BF_REQUIRE(lengths && ((kCache && vCache && weights) || capacity == 0) && ((kOut && vOut && weightsOut) || budget == 0), "NULL pointer");
     const bool inPlace = kOut == kCache;
-    BF_REQUIRE((vOut == vCache) == inPlace && (weightsOut == weights) == inPlace, "keys, values and weights go in place together or not at all");
-    BF_REQUIRE(!inPlace || outCapacity == capacity, "a call in place keeps the capacity");
+    // (of caches without rows only the lengths are left to write)
+    BF_REQUIRE(capacity == 0 || ((vOut == vCache) == inPlace && (weightsOut == weights) == inPlace),
+               "keys, values and weights go in place together or not at all");
+    BF_REQUIRE(capacity == 0 || !inPlace || outCapacity == capacity, "a call in place keeps the capacity");
     EvictParams p{};
     p.k = kCache; p.v = vCache; p.weights = weights; p.lengths = lengths; p.kOut = kOut; p.vOut = vOut; p.weightsOut = weightsOut;
     p.lengthsOut = lengthsOut; p.batch = int(batch); p.groups = int(groups); p.capacity = int(capacity); p.outCapacity = int(outCapacity);

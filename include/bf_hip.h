@@ -512,7 +512,7 @@ int bf_hip_attention_key_weights(const float* q, const float* k, const float* m,
  * rows that remain is left as it was.  kOut, vOut and weightsOut may be kCache, vCache and weights themselves, all three
  * together (outCapacity = capacity then).  lengthsOut (may be NULL, may be lengths) receives min(lengths, budget); kept
  * [batch, groups, budget] (may be NULL) the kept rows' old places.  Layers that share `lengths`: pass lengthsOut = NULL
- * for all but the last. */
+ * for all but the last.  With a headDim of 0 there is nothing to keep or cut and nothing is written. */
 int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weights, const int* lengths, float* kOut, float* vOut, float* weightsOut,
                     int* lengthsOut, int* kept, size_t batch, size_t kvHeads, size_t groups, size_t headDim, size_t capacity, size_t outCapacity,
                     size_t budget, size_t recent, bf_stream_t stream);

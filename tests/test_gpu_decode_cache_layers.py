@@ -38,3 +38,19 @@ def test_the_cpp_layer_cuts_all_layers_or_none(hip):
     assert os.path.exists(exe), "blackforge_amd/host has not been built"
     proc = subprocess.run([exe], capture_output=True, text=True, timeout=120)
     assert proc.returncode == 0, proc.stdout + proc.stderr
+
+
+@pytest.mark.parametrize("budget", [0, 5])
+def test_eviction_from_caches_without_rows_still_cuts_the_lengths(hip, budget):
+    """No capacity, so no sequence has rows, whatever its length says: lengthsOut is 0, the result's tensors stay as they were."""
+    D, batch, kv, hd = hip.DeviceTensor, 3, 2, 32
+    before = [np.full(s, 7, f32) for s in ((batch, 8, kv * hd), (batch, 8, kv * hd), (batch, kv, 8))]
+    out = [D.fromHost(x) for x in before]
+    lengths, left, kept = ints(hip, [4, 0, -2]), ints(hip, [9, 9, 9]), ints(hip, np.full((batch, kv, max(budget, 1)), 9))
+    hip.capi.call("bf_hip_kv_evict", None, None, None, lengths.ptr, *(t.ptr for t in out), left.ptr, kept.ptr, batch, kv, kv, hd, 0, 8, budget, 0, None)
+    assert left.toHostInts().tolist() == [0, 0, 0] and lengths.toHostInts().tolist() == [4, 0, -2]
+    assert (kept.toHostInts() == 9).all()
+    for t, x in zip(out, before):
+        assert t.toHost().tobytes() == x.tobytes()
+    hip.capi.call("bf_hip_kv_evict", None, None, None, lengths.ptr, *(t.ptr for t in out), lengths.ptr, None, batch, kv, kv, hd, 0, 8, budget, 0, None)
+    assert lengths.toHostInts().tolist() == [0, 0, 0]
