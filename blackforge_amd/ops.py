@@ -663,7 +663,8 @@ def treeAccept(logits, tokens, parents, counts=None) -> AcceptedPath:
              "treeAccept: expected logits [batch, nodes, vocab], tokens and 32-bit parents [batch, nodes]")
     batch, nodes, vocab = logits.shape
     _require(counts is None or _ints(counts, (batch,)), "treeAccept: one 32-bit count per sequence")
-    res = AcceptedPath(DeviceTensor((batch, nodes)), DeviceTensor((batch,)), DeviceTensor.zeros((batch,)))
+    make = DeviceTensor if nodes > 0 else DeviceTensor.zeros     # a call without nodes writes nothing: no node is accepted
+    res = AcceptedPath(DeviceTensor((batch, nodes)), make((batch,)), DeviceTensor.zeros((batch,)))
     _call("bf_hip_tree_accept", logits.ptr, tokens.ptr, parents.ptr, _pointer(counts), res.path.ptr, res.counts.ptr, res.next.ptr, batch, nodes, vocab,
           None)
     return res

@@ -521,7 +521,7 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
  * node's logits [batch, nodes, vocab].  tokens: float ids [batch, nodes]; parents [batch, nodes], each before its child
  * (a root's own parent is ignored); counts NULL: all nodes.  path [batch, nodes] receives the accepted nodes and then -1,
  * pathCounts[b] their number (0 if counts[b] is 0), next[b] the token chosen after the last of them, as a float id.  A
- * NaN is never chosen unless it is element 0 (argmax_last_position's rule).  vocab <= 2^24. */
+ * NaN is never chosen unless it is element 0 (argmax_last_position's rule).  vocab <= 2^24.  With `nodes` 0 nothing is written. */
 int bf_hip_tree_accept(const float* logits, const float* tokens, const int* parents, const int* counts, int* path, int* pathCounts, float* next,
                        size_t batch, size_t nodes, size_t vocab, bf_stream_t stream);
 /* The accepted nodes' keys and values appended to the caches of all layers: row path[b, i] of kNew, vNew (of every layer,

@@ -142,6 +142,7 @@ inline AcceptedPath treeAccept(const DeviceTensor& logits, const DeviceTensor& t
                 (counts == nullptr || counts->size() == logits.dim(0)), "treeAccept: needs logits [batch, nodes, vocab] and a token and a parent per node");
     const std::size_t batch = logits.dim(0), nodes = logits.dim(1);
     AcceptedPath r{DeviceArray<int>(batch * nodes), DeviceArray<int>(batch), DeviceTensor::zeros({batch})};
+    if (nodes == 0) check(bf_hip_fill_zero(r.counts.data(), batch * sizeof(int), nullptr));   // the call writes nothing: no node is accepted
     check(bf_hip_tree_accept(logits.data(), tokens.data(), parents.data(), counts != nullptr ? counts->data() : nullptr, r.path.data(), r.counts.data(),
                              r.next.data(), batch, nodes, logits.dim(2), nullptr));
     return r;

@@ -74,6 +74,11 @@ int main() {
     refused("a budget past the capacity", keep, 31);
     refused("more recent rows than the budget", keep, 12, 13);
     refused("no heads", keep, 12, 3, 0);
+
+    // a draft without nodes: none is accepted, whatever the counts' memory held before
+    { const hip::DeviceArray<int> dirty(std::vector<int>{9, 9, 9}); }
+    const auto accepted = hip::treeAccept(DeviceTensor({3, 0, 50}), DeviceTensor({3, 0}), hip::DeviceArray<int>(0));
+    expect(accepted.counts.toHost() == std::vector<int>({0, 0, 0}), "treeAccept without nodes");
     std::printf(failures == 0 ? "all passed\n" : "%d failed\n", failures);
     return failures != 0;
 }

@@ -54,3 +54,15 @@ def test_eviction_from_caches_without_rows_still_cuts_the_lengths(hip, budget):
         assert t.toHost().tobytes() == x.tobytes()
     hip.capi.call("bf_hip_kv_evict", None, None, None, lengths.ptr, *(t.ptr for t in out), lengths.ptr, None, batch, kv, kv, hd, 0, 8, budget, 0, None)
     assert lengths.toHostInts().tolist() == [0, 0, 0]
+
+
+def test_a_draft_without_nodes_accepts_none(hip):
+    """The counts are 0, whatever their memory held before, and an append of nothing leaves the lengths alone."""
+    D, batch = hip.DeviceTensor, 3
+    dirty = ints(hip, [9] * batch)
+    del dirty      # its block is the pool's next of this size
+    taken = hip.ops.treeAccept(D((batch, 0, 50)), D((batch, 0)), D((batch, 0)))
+    assert taken.counts.toHostInts().tolist() == [0] * batch and taken.next.toHost().tolist() == [0] * batch
+    cache, lengths = D.zeros((batch, 4, 8)), ints(hip, [1, 4, 0])
+    hip.ops.kvCommit([cache], [cache], [D((batch, 0, 8))], [D((batch, 0, 8))], taken, lengths)
+    assert lengths.toHostInts().tolist() == [1, 4, 0]
