@@ -617,6 +617,14 @@ __global__ void __launch_bounds__(256) rowWeightsKernel(TreeParams p, TilePlan p
     p.weightsOut[at] = block != 0 && p.weightsIn ? p.weightsIn[at] + all : all;
 }
 
+// A step without new tokens: the weights of the rows in use carried over (zeros without weightsIn).
+__global__ void __launch_bounds__(256) carryWeightsKernel(TreeParams p) {
+    const int j = int(blockIdx.x) * 256 + int(threadIdx.x), g = blockIdx.y, b = blockIdx.z;
+    if (j >= rowsInUse(p, b)) return;
+    const size_t at = (size_t(b) * p.groups + g) * p.capacity + j;
+    p.weightsOut[at] = p.weightsIn ? p.weightsIn[at] : 0.0f;
+}
+
 // The chunks of a row put together.  LPR lanes hold a row's columns, four each.  Few chunks a row (MANY false): every LPR
 // lanes have a row of their own and take its chunks in turn, so that few wavefronts wait out the chain of loads (24000 rows
 // of three chunks: 15 us with a wavefront each).  Many: a workgroup a row, 256 / LPR chunks at once.  Workgroups past
@@ -1088,7 +1096,16 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     if (st != BF_OK) return st;
     if (nodes > 64) return failInvalid(fn, "a tree has at most 64 nodes, got " + std::to_string(nodes));
     if (batch >= (size_t(1) << 16) || capacity >= (size_t(1) << 30)) return failInvalid(fn, "shape too large");
-    if (batch == 0 || nodes == 0 || headDim == 0) return BF_OK;
+    if (batch == 0) return BF_OK;
+    if (nodes == 0 || headDim == 0) {
+        if (!weights || capacity == 0) return BF_OK;
+        if (!p.lengths || !p.weightsOut) return failInvalid(fn, "NULL pointer");
+        if (p.weightsIn == p.weightsOut) return BF_OK;
+        p.groups = int(groups); p.capacity = int(capacity);
+        carryWeightsKernel<<<dim3(unsigned((capacity + 255) / 256), unsigned(groups), unsigned(batch)), 256, 0, asStream(stream)>>>(p);
+        BF_LAUNCH_CHECK();
+        return BF_OK;
+    }
     if (!p.q || !p.kNew || !p.vNew || !p.lengths || !p.out || (capacity != 0 && (!p.k || !p.v)) || (weights && capacity != 0 && !p.weightsOut))
         return failInvalid(fn, "NULL pointer");
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.nodes = int(nodes);

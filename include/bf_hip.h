@@ -479,7 +479,7 @@ int bf_hip_counter_add(int* counter, int by, bf_stream_t stream);
  * each may be NULL.  A node that sees nothing, or nothing but scores of -infinity, gets out = 0, l = 0 (m = -infinity).
  * Nodes i >= counts[b] are neither read nor written, and neither are rows that a node does not see: what lies there may
  * be NaN; a value that is not finite makes the outputs of the nodes that see it not finite.  Any alignment; 16-byte
- * aligned operands with headDim a multiple of 4 are faster. */
+ * aligned operands with headDim a multiple of 4 are faster.  With a headDim of 0 nothing is written. */
 int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
                           const int* counts, const uint64_t* visible, float* out, float* m, float* l, size_t batch, size_t heads, size_t kvHeads,
                           size_t nodes, size_t capacity, size_t headDim, float scale, bf_stream_t stream);
@@ -488,8 +488,9 @@ int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, 
  * divide kvHeads.  weights: [batch, groups, capacity].  For j < lengths[b] weightsOut[b, g, j] = weightsIn[b, g, j] + the
  * weight received; the new rows' weights follow at j = lengths[b] + node (where the row will be once it is appended) as far
  * as the capacity goes, without weightsIn; entries past them stay as they were.  weightsIn may be NULL (zeros) or be
- * weightsOut itself.  Takes a workspace of 4 bytes for every row of the cache, node and query head from the pool where that
- * is at most 1 GiB, or nodes * heads / kvHeads at most 16; else the products are made a second time. */
+ * weightsOut itself; with `nodes` or headDim 0 no row receives any.  Takes a workspace of 4 bytes for every row of the cache,
+ * node and query head from the pool where that is at most 1 GiB, or nodes * heads / kvHeads at most 16; else the products
+ * are made a second time. */
 int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
                                   const int* counts, const uint64_t* visible, float* out, float* m, float* l, const float* weightsIn,
                                   float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t nodes, size_t capacity,

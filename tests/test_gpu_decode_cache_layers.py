@@ -66,3 +66,21 @@ def test_a_draft_without_nodes_accepts_none(hip):
     cache, lengths = D.zeros((batch, 4, 8)), ints(hip, [1, 4, 0])
     hip.ops.kvCommit([cache], [cache], [D((batch, 0, 8))], [D((batch, 0, 8))], taken, lengths)
     assert lengths.toHostInts().tolist() == [1, 4, 0]
+
+
+@pytest.mark.parametrize("nodes,hd", [(0, 64), (3, 0), (0, 0)])
+def test_a_step_without_new_tokens_carries_the_weights(hip, rng, nodes, hd):
+    """No node or no column: no row receives any weight, so those in use have what they had, and the others stay as they were."""
+    D, batch, heads, groups, cap = hip.DeviceTensor, 3, 4, 2, 700
+    lengths = [700, 0, 257]
+    before = rng.random((batch, groups, cap)).astype(f32)
+    q, cache, w_in, dl = D((batch, nodes, heads * hd)), D((batch, cap, heads * hd)), D.fromHost(before), ints(hip, lengths)
+    for weights_in in (w_in, None):
+        out = D.fromHost(np.full(before.shape, 7, f32))
+        hip.capi.call("bf_hip_attention_tree_weights", q.ptr, q.ptr, q.ptr, cache.ptr, cache.ptr, dl.ptr, None, None, q.ptr, None, None,
+                      weights_in.ptr if weights_in else None, out.ptr, batch, heads, heads, groups, nodes, cap, hd, 0.125, None)
+        used = np.arange(cap) < np.array(lengths)[:, None, None]
+        np.testing.assert_array_equal(out.toHost(), np.where(used, before if weights_in else np.zeros_like(before), f32(7)))
+    hip.capi.call("bf_hip_attention_tree_weights", q.ptr, q.ptr, q.ptr, cache.ptr, cache.ptr, dl.ptr, None, None, q.ptr, None, None,
+                  w_in.ptr, w_in.ptr, batch, heads, heads, groups, nodes, cap, hd, 0.125, None)
+    np.testing.assert_array_equal(w_in.toHost(), before)
