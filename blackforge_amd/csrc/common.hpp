@@ -62,6 +62,10 @@ constexpr int kWave = 64;            // CDNA wavefront
 constexpr int kBlock = 256;          // 4 waves: one per SIMD of a CU
 constexpr unsigned kMaxGridX = 1u << 20;
 
+// A launch has less than 2^32 work-items along x: workgroups there may be with `threads` each.  Checked before the first
+// launch of a call whose grid grows with its shape, so that none is refused behind others that have run.
+constexpr size_t mostBlocks(size_t threads) { return ((size_t(1) << 32) - 1) / threads; }
+
 inline unsigned gridFor(size_t work, size_t perBlock, unsigned cap = kMaxGridX) {
     size_t blocks = (work + perBlock - 1) / perBlock;
     if (blocks < 1) blocks = 1;

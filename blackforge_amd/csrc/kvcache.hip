@@ -381,6 +381,12 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
     p.k = kCache; p.v = vCache; p.weights = weights; p.lengths = lengths; p.kOut = kOut; p.vOut = vOut; p.weightsOut = weightsOut;
     p.lengthsOut = lengthsOut; p.batch = int(batch); p.groups = int(groups); p.capacity = int(capacity); p.outCapacity = int(outCapacity);
     p.budget = int(budget); p.recent = int(recent); p.slab = int(kvHeads / groups * headDim);
+    const bool vec = p.slab % 4 == 0 && aligned16(kCache) && aligned16(vCache) && aligned16(kOut) && aligned16(vOut);
+    const int slices = std::max(1, (p.slab / (vec ? 4 : 1) + 15) / 16);
+    const size_t tiles = std::max<size_t>(1, (std::min(budget, capacity) + 127) / 128);
+    const int splits = inPlace ? 1 : int(std::min<size_t>(tiles, 64));
+    const size_t gridX = size_t(slices) * 2 * size_t(splits);
+    BF_REQUIRE(batch * groups <= mostBlocks(1024) && gridX <= mostBlocks(256), "shape too large");
     hipStream_t s = asStream(stream);
     const size_t keptInts = kept ? 0 : batch * groups * budget;
     Scratch own((batch + keptInts) * sizeof(int));
@@ -393,11 +399,7 @@ int bf_hip_kv_evict(const float* kCache, const float* vCache, const float* weigh
     else if (capacity <= 64 * 1024) evictSelectKernel<64><<<pairs, 1024, 0, s>>>(p);
     else evictSelectKernel<0><<<pairs, 1024, 0, s>>>(p);
     BF_LAUNCH_CHECK();
-    const bool vec = p.slab % 4 == 0 && aligned16(kCache) && aligned16(vCache) && aligned16(kOut) && aligned16(vOut);
-    const int slices = std::max(1, (p.slab / (vec ? 4 : 1) + 15) / 16);
-    const size_t tiles = std::max<size_t>(1, (std::min(budget, capacity) + 127) / 128);
-    const int splits = inPlace ? 1 : int(std::min<size_t>(tiles, 64));
-    const dim3 grid(unsigned(slices) * 2 * unsigned(splits), unsigned(groups), unsigned(batch));
+    const dim3 grid{unsigned(gridX), unsigned(groups), unsigned(batch)};
     // rows that stream past the last-level cache carry the non-temporal hint (0.9 GB moved: 195 -> 185 us with the selection)
     const size_t moved = batch * std::min(budget, capacity) * groups * size_t(p.slab) * 4 * sizeof(float);
     if (vec && streamsPastCache(moved)) evictMoveKernel<4, true><<<grid, 256, 0, s>>>(p, slices, splits);

@@ -983,12 +983,16 @@ int launchKeySplit(const KeyWeightParams& p, int mode, size_t grid, hipStream_t 
     return BF_OK;
 }
 
-int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
+// many queries: bound by the products, which the bf16 route does faster; few: by reading the keys
+bool splitProducts(const KeyWeightParams& p) { return paddedHeadDim(size_t(p.hd)) <= 128 && p.newLen > 64; }
+int keysPerBlock(const KeyWeightParams& p) {
     const int hdp = paddedHeadDim(size_t(p.hd));
-    // many queries: bound by the products, which the bf16 route does faster; few: by reading the keys
-    const bool split = hdp <= 128 && p.newLen > 64;
-    const int keysPerBlock = (hdp > 128 || (split && hdp == 128) ? 2 : 4) * 64;
-    p.keyBlocks = (p.totalLen + keysPerBlock - 1) / keysPerBlock;
+    return (hdp > 128 || (splitProducts(p) && hdp == 128) ? 2 : 4) * 64;
+}
+
+// The chunks of queries; a shape too large is refused here, before anything is launched
+int planKeyWeights(const char* fn, KeyWeightParams& p) {
+    p.keyBlocks = (p.totalLen + keysPerBlock(p) - 1) / keysPerBlock(p);
     const size_t pairs = size_t(p.batch) * p.heads, blocks = pairs * p.keyBlocks;
     // Queries a workgroup walks: as many as leave three workgroups a compute unit (8 prompts of 1024 tokens, 12 heads: 62, 56, 53,
     // 67 us with 128, 256, 512, 1024; one of 4096: 101, 95, 92, 158 with 256 to 2048)
@@ -997,8 +1001,13 @@ int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
     while (chunk < p.newLen && chunk < (1 << 30) && pairs * size_t((p.newLen + chunk - 1) / chunk) * p.totalLen > (size_t(1) << 28)) chunk *= 2;   // sums of 1 GiB
     p.queryChunk = chunk;
     p.queryChunks = std::max(1, (p.newLen + chunk - 1) / chunk);
-    const size_t grid = blocks * p.queryChunks;
-    if (grid >= (size_t(1) << 31)) return failInvalid(fn, "shape too large");
+    return blocks * p.queryChunks > mostBlocks(256) ? failInvalid(fn, "shape too large") : BF_OK;
+}
+
+int keyWeights(KeyWeightParams p, hipStream_t s) {
+    const int hdp = paddedHeadDim(size_t(p.hd));
+    const bool split = splitProducts(p);
+    const size_t pairs = size_t(p.batch) * p.heads, grid = pairs * p.keyBlocks * p.queryChunks;
     Scratch part(pairs * p.queryChunks * p.totalLen * sizeof(float));
     if (part.status != BF_OK) return part.status;
     p.part = part.as<float>();
@@ -1016,7 +1025,7 @@ int keyWeights(const char* fn, KeyWeightParams p, hipStream_t s) {
         }
         if (st != BF_OK) return st;
     }
-    keyWeightJoinKernel<<<dim3(unsigned((p.totalLen + 255) / 256), unsigned(p.groups), unsigned(p.batch)), 256, 0, s>>>(p, keysPerBlock);
+    keyWeightJoinKernel<<<dim3(unsigned((p.totalLen + 255) / 256), unsigned(p.groups), unsigned(p.batch)), 256, 0, s>>>(p, keysPerBlock(p));
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
@@ -1073,11 +1082,14 @@ int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, size_t 
     BF_LAUNCH_CHECK();
     return BF_OK;
 }
+int joinLanes(size_t hd) { return hd <= 32 ? 8 : hd <= 64 ? 16 : hd <= 128 ? 32 : 64; }
 int launchJoin(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
-    if (p.hd <= 32) return launchJoinOf<8>(p, plan, rows, weightBlocks, s);
-    if (p.hd <= 64) return launchJoinOf<16>(p, plan, rows, weightBlocks, s);
-    if (p.hd <= 128) return launchJoinOf<32>(p, plan, rows, weightBlocks, s);
-    return launchJoinOf<64>(p, plan, rows, weightBlocks, s);
+    switch (joinLanes(size_t(p.hd))) {
+        case 8: return launchJoinOf<8>(p, plan, rows, weightBlocks, s);
+        case 16: return launchJoinOf<16>(p, plan, rows, weightBlocks, s);
+        case 32: return launchJoinOf<32>(p, plan, rows, weightBlocks, s);
+        default: return launchJoinOf<64>(p, plan, rows, weightBlocks, s);
+    }
 }
 
 int checkHeads(const char* fn, size_t heads, size_t kvHeads, size_t groups, size_t headDim) {
@@ -1161,8 +1173,19 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const bool apart = recompute || (keepScores && kvHeads / groups * rows > 4);
     plan.keyBlocks = !keepScores ? 1 : apart ? int((capacity + 63) / 64) + 1 : int((capacity + 1023) / 1024);
     const size_t weightBlocks = weights && capacity != 0 ? batch * groups * size_t(plan.keyBlocks) : 0;
-    if (rowsAll + weightBlocks >= (size_t(1) << 31) || size_t(plan.items) * kvHeads * size_t(plan.rowGroups) >= (size_t(1) << 31))
+    const size_t grid = (size_t(plan.items) * kvHeads + 7) / 8 * 8 * size_t(plan.rowGroups);
+    // (a workgroup a row joins where there are few rows only)
+    const size_t joinBlocks = join ? (rowsAll * size_t(joinLanes(headDim)) + 255) / 256 : 0;
+    if (grid > mostBlocks(256) || joinBlocks > mostBlocks(256) || joinBlocks * !apart + weightBlocks > mostBlocks(256))
         return failInvalid(fn, "shape too large");
+    KeyWeightParams w{};
+    if (recompute) {
+        w.q = p.q; w.k = p.k; w.counts = p.counts; w.lengths = p.lengths; w.weightsIn = p.weightsIn; w.weightsOut = p.weightsOut;
+        w.batch = p.batch; w.heads = p.heads; w.kvHeads = p.kvHeads; w.groups = p.groups; w.newLen = p.nodes; w.totalLen = p.capacity;
+        w.kvRows = p.capacity; w.hd = p.hd; w.oldLen = p.capacity; w.weightRows = p.capacity; w.scale = p.scale;
+        st = planKeyWeights(fn, w);
+        if (st != BF_OK) return st;
+    }
     const size_t need[] = {join || (weights && !apart) ? slots * sizeof(float4v) : 0, join ? slots * plan.partPitch * sizeof(float) : 0, batch * sizeof(int2),
                            keepScores ? rowsAll * size_t(plan.scorePitch) * sizeof(float) : 0, weights ? rowsAll * 64 * sizeof(float) : 0,
                            recompute && !(p.m && p.l) ? 2 * rowsAll * sizeof(float) : 0, apart ? rowsAll * sizeof(float2) : 0};
@@ -1185,9 +1208,8 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
         if (!p.m) p.m = own2;
         if (!p.l) p.l = own2 + rowsAll;
     }
-    const unsigned grid = unsigned((size_t(plan.items) * kvHeads + 7) / 8 * 8 * size_t(plan.rowGroups));
     const int mode = headDim % 4 != 0 || !aligned16({p.q, p.kNew, p.vNew, p.k, p.v, p.out}) ? 0 : headDim == size_t(hdp) ? 2 : 1;
-    st = launchTiles(p, plan, hdp, rt, mode, grid, s);
+    st = launchTiles(p, plan, hdp, rt, mode, unsigned(grid), s);
     if (st != BF_OK) return st;
     // the new rows' weights, and the cached rows' where their dot products were kept, ride on the launch that joins
     st = launchJoin(p, plan, rowsAll, apart ? 0 : weightBlocks, s);
@@ -1197,11 +1219,8 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
         BF_LAUNCH_CHECK();
     }
     if (recompute) {
-        KeyWeightParams w{};
-        w.q = p.q; w.k = p.k; w.m = p.m; w.l = p.l; w.counts = p.counts; w.lengths = p.lengths; w.weightsIn = p.weightsIn; w.weightsOut = p.weightsOut;
-        w.batch = p.batch; w.heads = p.heads; w.kvHeads = p.kvHeads; w.groups = p.groups; w.newLen = p.nodes; w.totalLen = p.capacity;
-        w.kvRows = p.capacity; w.hd = p.hd; w.oldLen = p.capacity; w.weightRows = p.capacity; w.scale = p.scale;
-        return keyWeights(fn, w, s);
+        w.m = p.m; w.l = p.l;
+        return keyWeights(w, s);
     }
     return BF_OK;
 }
@@ -1249,7 +1268,8 @@ int bf_hip_attention_key_weights(const float* q, const float* k, const float* m,
     p.batch = int(batch); p.heads = int(heads); p.kvHeads = int(kvHeads); p.groups = int(groups); p.newLen = headDim == 0 ? 0 : int(newLen);
     p.totalLen = int(totalLen); p.kvRows = int(kvRows); p.hd = int(headDim); p.oldLen = int(oldLen); p.weightRows = int(weightRows);
     p.scale = scale;
-    return keyWeights(__func__, p, asStream(stream));
+    st = planKeyWeights(__func__, p);
+    return st != BF_OK ? st : keyWeights(p, asStream(stream));
 }
 
 }  // extern "C"

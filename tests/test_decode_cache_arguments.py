@@ -4,6 +4,8 @@ import ctypes
 
 import pytest
 
+from test_decode_cache_refusals import EVICT, KEYS, TREE, WEIGHTS
+
 A = 1 << 20   # stands for any device address
 
 
@@ -159,3 +161,18 @@ def test_eviction_refuses_budgets_and_lists_that_do_not_fit(calls):
     with pytest.raises(ValueError, match="kvEvict"):
         ops.kvEvict(k, v, w, tensor(2), 7, 12, 3)
     assert calls == []
+
+
+@pytest.mark.parametrize("entry,base,change", [
+    ("bf_hip_attention_tree", TREE, dict(batch=60000, heads=512, kvHeads=512, nodes=1)),                                     # row tiles
+    ("bf_hip_attention_tree_weights", WEIGHTS, dict(batch=4000, heads=64, kvHeads=64, groups=64, nodes=16, capacity=1 << 13)),   # blocks of keys
+    ("bf_hip_attention_tree_weights", WEIGHTS, dict(batch=16, heads=4096, kvHeads=1, groups=1, nodes=64, capacity=1 << 17)),  # products made again
+    ("bf_hip_attention_key_weights", KEYS, dict(batch=60000, heads=512, kvHeads=512)),
+    ("bf_hip_kv_evict", EVICT, dict(batch=60000, kvHeads=512, groups=512)),                                                  # selections
+    ("bf_hip_kv_evict", EVICT, dict(kvHeads=1, groups=1, headDim=(1 << 24) - 1, capacity=8192, outCapacity=8192, budget=8192)),    # columns
+])
+def test_launches_too_large_are_refused_before_the_first(entry, base, change):
+    """Each of several launches of a call has less than 2^32 work-items; the check comes before any of them."""
+    from blackforge_amd import capi
+    with pytest.raises(ValueError, match="too large"):
+        capi.call(entry, *{**base, **change}.values())
