@@ -998,7 +998,7 @@ int planKeyWeights(const char* fn, KeyWeightParams& p) {
     // 67 us with 128, 256, 512, 1024; one of 4096: 101, 95, 92, 158 with 256 to 2048)
     int chunk = 2048;
     while (chunk > 128 && blocks * size_t((p.newLen + chunk - 1) / chunk) < size_t(computeUnits()) * 3) chunk /= 2;
-    while (chunk < p.newLen && chunk < (1 << 30) && pairs * size_t((p.newLen + chunk - 1) / chunk) * p.totalLen > (size_t(1) << 28)) chunk *= 2;   // sums of 1 GiB
+    while (chunk < p.newLen && chunk < (1 << 30) && pairs * size_t((p.newLen + chunk - 1) / chunk) * p.totalLen > (size_t(1) << 28)) chunk *= 2;   // sums of 1 GiB, or one chunk's
     p.queryChunk = chunk;
     p.queryChunks = std::max(1, (p.newLen + chunk - 1) / chunk);
     return blocks * p.queryChunks > mostBlocks(256) ? failInvalid(fn, "shape too large") : BF_OK;
@@ -1125,9 +1125,11 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     const size_t share = heads / kvHeads, rows = nodes * share;
     // The weights come from the dot products that the pass leaves in a workspace, up to 1 GiB of it (or 64 bytes a key and key
     // head); past that they are made again from the keys (20 nodes over 4 x 8192 rows, 8 heads of 64: 50 us against 66; 64
-    // nodes 78 against 97; 512 rows to a key head 484 against 514).
+    // nodes 78 against 97; 512 rows to a key head 484 against 514), which takes sums of 4 bytes a key and query head, one part
+    // in `nodes` of what is kept: with three nodes or fewer that saves too little (one node over 500000 rows, 128 heads on one
+    // key head of 128: 0.39 ms kept, 5.0 made again; three 1.2 and 5.8; 32 heads on one of 64, 1000000 rows: 0.20 and 1.4).
     const size_t scoreBytes = batch * kvHeads * rows * ((capacity + 15) / 16 * 16) * sizeof(float);
-    const bool keepScores = weights && capacity != 0 && (rows <= 16 || scoreBytes <= size_t(1) << 30);
+    const bool keepScores = weights && capacity != 0 && (nodes <= 3 || rows <= 16 || scoreBytes <= size_t(1) << 30);
     const bool recompute = weights && capacity != 0 && !keepScores;
     // Row tiles a wavefront holds: what the rows fill, up to the registers there are (two tiles of 192 columns halve the reads, 142
     // -> 90 us for 17 nodes over 4 x 8192 rows, 8 heads; of 256 they spill, 195 -> 324).  With less to do, two at most, and one

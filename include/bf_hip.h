@@ -489,8 +489,8 @@ int bf_hip_attention_tree(const float* q, const float* kNew, const float* vNew, 
  * weight received; the new rows' weights follow at j = lengths[b] + node (where the row will be once it is appended) as far
  * as the capacity goes, without weightsIn; entries past them stay as they were.  weightsIn may be NULL (zeros) or be
  * weightsOut itself; with `nodes` or headDim 0 no row receives any.  Takes a workspace of 4 bytes for every row of the cache,
- * node and query head from the pool where that is at most 1 GiB, or nodes * heads / kvHeads at most 16; else the products
- * are made a second time. */
+ * node and query head from the pool where that is at most 1 GiB, or `nodes` at most 3, or nodes * heads / kvHeads at most 16;
+ * else the products are made a second time, with a workspace of 4 bytes for every row of the cache and query head. */
 int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float* vNew, const float* kCache, const float* vCache, const int* lengths,
                                   const int* counts, const uint64_t* visible, float* out, float* m, float* l, const float* weightsIn,
                                   float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t nodes, size_t capacity,
@@ -501,7 +501,8 @@ int bf_hip_attention_tree_weights(const float* q, const float* kNew, const float
  * with j <= oldLen + i of exp(score_ij - m_i) / l_i, for j < totalLen; weights: [batch, groups, weightRows].  A row with
  * l = 0 gives nothing.  weightsIn may be NULL (zeros) or weightsOut itself.  oldLen >= totalLen - 1: no causal mask.
  * The q and k that count must be finite: past 64 queries the products are made of bf16 terms, which infinities have none;
- * a query whose m or l is NaN makes the weights of the keys it sees NaN. */
+ * a query whose m or l is NaN makes the weights of the keys it sees NaN.  Takes a workspace of 4 bytes for every key, query
+ * head and chunk of queries, at most 1 GiB if more than one chunk is needed. */
 int bf_hip_attention_key_weights(const float* q, const float* k, const float* m, const float* l, const int* counts, const float* weightsIn,
                                  float* weightsOut, size_t batch, size_t heads, size_t kvHeads, size_t groups, size_t newLen, size_t totalLen,
                                  size_t kvRows, size_t headDim, float scale, size_t oldLen, size_t weightRows, bf_stream_t stream);

@@ -1,11 +1,12 @@
 """GPU tests of the cache operators over several layers that share their sequences' lengths, and at sizes with nothing in them."""
+import ctypes
 import os
 import subprocess
 
 import numpy as np
 import pytest
 
-from test_gpu_decode_cache import ints, kept_rows
+from test_gpu_decode_cache import check_tree, check_weights, ints, kept_rows, make, reference, run_tree, tree_masks
 
 pytestmark = pytest.mark.gpu
 f32 = np.float32
@@ -84,3 +85,37 @@ def test_a_step_without_new_tokens_carries_the_weights(hip, rng, nodes, hd):
     hip.capi.call("bf_hip_attention_tree_weights", q.ptr, q.ptr, q.ptr, cache.ptr, cache.ptr, dl.ptr, None, None, q.ptr, None, None,
                   w_in.ptr, w_in.ptr, batch, heads, heads, groups, nodes, cap, hd, 0.125, None)
     np.testing.assert_array_equal(w_in.toHost(), before)
+
+
+@pytest.mark.parametrize("stats", [True, False])
+@pytest.mark.parametrize("nodes", [1, 3, 4, 17])
+def test_weights_over_caches_whose_products_pass_a_gibibyte(hip, rng, nodes, stats):
+    """Many heads to a key head over a cache with room for 5 million rows: products kept (up to three nodes) and made again, on
+    statistics of the caller's or of the call's own; the workspace is what the header says."""
+    heads, hd, cap = 64, 4, 5_000_000
+    scale, lengths, counts = 0.5, [300], [nodes]
+    q, kn, vn, k, v = make(rng, 1, heads, 1, hd, nodes, 301, lengths, counts)
+    visible = tree_masks(rng, 1, nodes)
+    want = reference(q, kn, vn, k, v, lengths, counts, visible, heads, 1, 1, scale)
+    k, v = (np.concatenate([x, np.full((1, cap - 301, hd), np.nan, f32)], 1) for x in (k, v))
+    weights = rng.random((1, 1, cap)).astype(f32)
+    hip.capi.call("bf_hip_pool_trim")
+
+    def from_driver():
+        stats = hip.capi.PoolStats()
+        hip.capi.call("bf_hip_pool_stats", ctypes.byref(stats))
+        return stats.bytes_from_driver
+    before = from_driver()
+    got = run_tree(hip, q, kn, vn, k, v, lengths, counts, visible, heads, 1, scale, weights, 1, stats=stats)
+    taken = from_driver() - before
+    if stats:
+        check_tree(got, want, counts, 5.5, "past a gibibyte")
+    else:
+        assert (got[1] == 7).all() and (got[2] == 7).all()
+        check_tree((got[0], want[1], want[2]), want, counts, 5.5, "past a gibibyte without statistics")
+    check_weights(got[3], weights, want[3], lengths, counts, heads * nodes, want[4], "past a gibibyte")
+    del got
+    workspace = 4 * heads * cap * (nodes if nodes <= 3 else 1)
+    # operands and weights twice, 1/4 more at most for the pool's size classes, and 64 MiB for what grows with neither
+    assert taken <= 1.25 * (workspace + 4 * cap * (2 * hd + 2)) + (64 << 20), f"{taken / 2**20:.0f} MiB taken"
+    hip.capi.call("bf_hip_pool_trim")
