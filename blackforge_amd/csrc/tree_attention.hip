@@ -77,6 +77,7 @@ struct TilePlan {
 // slots times the length of a round, and neighbouring sizes differ much (32 equal sequences, 12 heads, 512 slots: three
 // chunks each are 1152 workgroups, 3 rounds of a third; four are 1536, 3 rounds of a quarter).  Lane c of the wavefront tries one
 // size, from half as much again as fills the slots once down to a third of it; the cheapest is taken, the larger on a tie.
+// Lane 0's makes slots / 1.5 + batch chunks at most, which `target`, 3 slots + batch, always has room for.
 __device__ __forceinline__ int bestChunk(const TreeParams& p, const TilePlan& plan, int length, int total) {
     const int lane = threadIdx.x & 63, mine = (length + 63) / 64;
     const float base = float(total) / plan.slots;            // units of 64 keys that fill the slots once
@@ -94,7 +95,7 @@ __device__ __forceinline__ int bestChunk(const TreeParams& p, const TilePlan& pl
         const int other = __shfl_xor(best, off, 64);
         if (otherCost < cost || (otherCost == cost && other > best)) { cost = otherCost; best = other; }
     }
-    return cost == INFINITY ? int(fminf(ceilf(base * 2.0f) + 1.0f, 16777216.0f)) : best;
+    return best;
 }
 
 // Chunk sizes from the lengths themselves: about `target` chunks of equal size over all sequences, at least one for each (a
