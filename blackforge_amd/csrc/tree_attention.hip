@@ -1074,8 +1074,13 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
 
 template <int LPR>
 int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
-    // few chunks a row on average, unless there are so few rows that their lanes would not fill the device
-    const bool many = size_t(plan.items) > size_t(p.batch) * (rows * LPR > size_t(computeUnits()) * 512 ? 32 : 4);
+    // A workgroup a row where there is room for more than four chunks a sequence, unless the rows' lanes alone fill the device twice
+    // (their sequences then have 17 chunks at most).  A workgroup each against lanes each: one node over 8000 rows, 8 heads of
+    // 64, 13 against 21 us, 64 nodes 21 and 24; 26 nodes over 120011 rows, 16 heads of 128, 322 and 333; more lanes than the
+    // bound: 64 nodes over 32 ragged sequences, 12 heads, 181 and 154, over 16 x 4000 rows, 8 heads of 128, 173 and 161.  Up to
+    // four chunks it is the same within 3 %; close below the bound the workgroups lose up to 10 % (64 nodes over 8 x 4000
+    // rows, 16 heads of 64: 101 and 91).
+    const bool many = size_t(plan.items) > size_t(p.batch) * 4 && rows * LPR <= size_t(computeUnits()) * 512;
     const size_t blocks = size_t(plan.items) == size_t(p.batch) ? 0 : many ? rows : (rows * LPR + 255) / 256;   // one chunk each: nothing to join
     if (blocks + weightBlocks == 0) return BF_OK;
     if (many) treeJoinKernel<LPR, true><<<unsigned(blocks + weightBlocks), 256, 0, s>>>(p, plan, unsigned(blocks));
