@@ -160,7 +160,9 @@ __global__ void __launch_bounds__(1024) evictSelectKernel(EvictParams p) {
 // the rows, of the keys or of the values, and takes tiles of 128 rows in order, `splits` workgroups dealing them out
 // among themselves when the result goes to other tensors (each tile is then on its own).  In place one workgroup walks
 // all the tiles: a tile's reads come before the barrier, its writes after it, and what later tiles read lies at or
-// after their own first row.
+// after their own first row.  That leaves few workgroups and a load's latency bare in every tile: 8 ragged sequences of up
+// to 16384 rows cut to 4096, 16 heads of 128, 335 us with the selection where the call to other tensors takes 186; one such
+// sequence 202 and 40.
 template <int VEC, bool NT>
 __global__ void __launch_bounds__(256) evictMoveKernel(EvictParams p, int slices, int splits) {
     constexpr int ROWS = 16, U = 8, TILE = ROWS * U;

@@ -53,8 +53,8 @@ __device__ __forceinline__ unsigned long long newRowsSeen(const TreeParams& p, i
 // the error of d is relative to d, not to the score.  The true maximum is kept beside it for the statistics.
 //
 // Measured: 26 nodes, 16 heads of 128, 120011 rows 322 us = 6.1 TB/s with the join (HBM); 32 ragged sequences of up to 4032 rows,
-// 12 heads of 64, 64 nodes 147 us (427 MB, 10.3 GFLOP: the matrix instruction, 62 % busy, and the start and end of a
-// workgroup, 15 us by themselves); one node over 701 rows 10 us (two dependent launches).
+// 12 heads of 64, 64 nodes 147 us (427 MB, 10.3 GFLOP: the matrix pipe is busy for half of the time, and the call takes 22 us
+// over empty caches, the start and end of a workgroup and the join); one node over 701 rows 10 us (two dependent launches).
 struct TilePlan {
     int target;          // chunks per (key head, group of row tiles) that the launch wants in total over the sequences
     int minChunk;        // keys a chunk has at least
@@ -162,7 +162,7 @@ __device__ __forceinline__ Chunk findChunk(const TreeParams& p, const TilePlan& 
 // Columns d .. of a row.  MODE 2: headDim == HDP, 16-byte aligned; 1: a multiple of 4, aligned; 0: anything.  `sure`: the
 // caller's form is for head dims that all have these columns.  With mode 1 the columns past the row's end hold any others of
 // it, and the caller takes them out where it uses them: a select behind a load waits for it (head dim 100, 4 x 8192 rows, 8
-// heads: 80 us with the select here, 59 without; 160: 135 and 111; one element at a time the select is better, 33: 36 and 42).
+// heads: 60 us with the select here, 48 without; 160: 100 and 72; one element at a time the select is better, 33: 34 and 40).
 template <int MODE, int W>
 __device__ __forceinline__ void fetchColumns(float (&x)[W], const float* row, int d, int hd, bool sure = false) {
     if constexpr (MODE == 0) {
@@ -1074,12 +1074,12 @@ int launchTiles(const TreeParams& p, const TilePlan& plan, int hdp, int rt, int 
 
 template <int LPR>
 int launchJoinOf(const TreeParams& p, const TilePlan& plan, size_t rows, size_t weightBlocks, hipStream_t s) {
-    // A workgroup a row where there is room for more than four chunks a sequence, unless the rows' lanes alone fill the device twice
-    // (their sequences then have 17 chunks at most).  A workgroup each against lanes each: one node over 8000 rows, 8 heads of
-    // 64, 13 against 21 us, 64 nodes 21 and 24; 26 nodes over 120011 rows, 16 heads of 128, 322 and 333; more lanes than the
-    // bound: 64 nodes over 32 ragged sequences, 12 heads, 181 and 154, over 16 x 4000 rows, 8 heads of 128, 173 and 161.  Up to
-    // four chunks it is the same within 3 %; close below the bound the workgroups lose up to 10 % (64 nodes over 8 x 4000
-    // rows, 16 heads of 64: 101 and 91).
+    // A workgroup a row where there is room for more than four chunks a sequence, unless the rows' lanes alone give every SIMD
+    // two wavefronts (their sequences then have 17 chunks at most).  A workgroup each against lanes each: one node over 8000
+    // rows, 8 heads of 64, 13 against 21 us, 64 nodes 21 and 24; 26 nodes over 120011 rows, 16 heads of 128, 322 and 333; more
+    // lanes than the bound: 64 nodes over 32 ragged sequences, 12 heads, 181 and 154, over 16 x 4000 rows, 8 heads of 128, 173
+    // and 161.  Up to four chunks it is the same within 5 %; close below the bound the workgroups lose up to 10 % (64 nodes
+    // over 8 x 4000 rows, 16 heads of 64: 101 and 91).
     const bool many = size_t(plan.items) > size_t(p.batch) * 4 && rows * LPR <= size_t(computeUnits()) * 512;
     const size_t blocks = size_t(plan.items) == size_t(p.batch) ? 0 : many ? rows : (rows * LPR + 255) / 256;   // one chunk each: nothing to join
     if (blocks + weightBlocks == 0) return BF_OK;
@@ -1130,19 +1130,20 @@ int treeAttention(const char* fn, TreeParams p, size_t batch, size_t heads, size
     p.capacity = int(capacity); p.hd = int(headDim);
     const size_t share = heads / kvHeads, rows = nodes * share;
     // The weights come from the dot products that the pass leaves in a workspace, up to 1 GiB of it (or 64 bytes a key and key
-    // head); past that they are made again from the keys (20 nodes over 4 x 8192 rows, 8 heads of 64: 50 us against 66; 64
-    // nodes 78 against 97; 512 rows to a key head 484 against 514), which takes sums of 4 bytes a key and query head, one part
+    // head); past that they are made again from the keys (20 nodes over 4 x 8100 rows, 8 heads of 64: 44 us against 60; 64
+    // nodes 72 against 95; 512 rows to a key head 481 against 510), which takes sums of 4 bytes a key and query head, one part
     // in `nodes` of what is kept: with three nodes or fewer that saves too little (one node over 500000 rows, 128 heads on one
     // key head of 128: 0.39 ms kept, 5.0 made again; three 1.2 and 5.8; 32 heads on one of 64, 1000000 rows: 0.20 and 1.4).
     const size_t scoreBytes = batch * kvHeads * rows * ((capacity + 15) / 16 * 16) * sizeof(float);
     const bool keepScores = weights && capacity != 0 && (nodes <= 3 || rows <= 16 || scoreBytes <= size_t(1) << 30);
     const bool recompute = weights && capacity != 0 && !keepScores;
-    // Row tiles a wavefront holds: what the rows fill, up to the registers there are (two tiles of 192 columns halve the reads, 142
-    // -> 90 us for 17 nodes over 4 x 8192 rows, 8 heads; of 256 they spill, 195 -> 324).  With less to do, two at most, and one
-    // where the tiles of all sequences are half the compute units at most: more workgroups, and each starts and ends sooner.  The
+    // Row tiles a wavefront holds: what the rows fill, up to the registers there are (two tiles of 192 columns halve the reads,
+    // 98 -> 90 us for 17 nodes over 4 x 8192 rows, 8 heads; of 256 they spill and take two thirds longer).  With less to do, two
+    // at most, and one where the tiles of all sequences are half the compute units at most: more workgroups, and each starts and ends sooner.  The
     // measure is keys (by the capacity) x row tiles x columns, 0.75 and 2 times 2^18 of them a compute unit.  53 nodes over 700 rows, 8
-    // heads of 64: 11, 14, 19 us with one, two, four; over 30000 rows 49, 51, 54; over 10 x 2000 55, 48, 51; 64 nodes over 32
-    // ragged sequences, 12 heads: 188, 155, 147; heads of 128, 24 nodes over 3 x 8000 rows: 52, 56, 53 nodes 87, 76.
+    // heads of 64: 12, 14, 19 us with one, two, four; over 30000 rows 48, 51, 53; over 10 x 2000 55, 49, 50; 64 nodes over 32
+    // ragged sequences, 12 heads: 193, 157, 154; heads of 128, 24 nodes over 3 x 8000 rows: 43, 50, 53 nodes 79, 73.  Lengths far
+    // below the capacity are not known here: 64 nodes over 4 x 256 rows of room for 8192, 8 heads of 64: 15, 18, 24 us.
     const int hdp = headDim > 64 && headDim <= 96 ? 96 : paddedHeadDim(headDim);
     const size_t device = size_t(computeUnits()), tiles = batch * kvHeads * ((rows + 15) / 16);
     const double work = double(tiles) * double(capacity) * hdp / double(device << 18);
